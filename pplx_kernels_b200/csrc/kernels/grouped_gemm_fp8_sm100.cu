@@ -38,6 +38,7 @@
 #include "../core/device_utils.cuh"
 #include "../core/ptx.cuh"
 #include "../core/tcgen05.cuh"
+#include "../core/tensor_map.h"
 #include "../core/utils.h"
 #include "../core/wait.cuh"
 #include "a2a_device.cuh"
@@ -87,23 +88,6 @@ struct Fp8GemmArgs {
 namespace pplx {
 namespace {
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fp8() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    PPLX_CHECK(q == cudaDriverEntryPointSuccess && p != nullptr,
-               "cuTensorMapEncodeTiled is not available in this driver");
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
 // [experts, rows, k] one-byte elements with k contiguous; tiles of 128 B x 128 rows x 1,
 // 128-byte swizzle, out-of-range elements read as zero.
 CUtensorMap make_byte_map(const void* base, int64_t experts, int64_t rows, int64_t k,
@@ -111,19 +95,12 @@ CUtensorMap make_byte_map(const void* base, int64_t experts, int64_t rows, int64
   PPLX_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride_row % 16 == 0 &&
                  stride_expert % 16 == 0,
              "fp8 operands must be 16-byte aligned with strides that are multiples of 16");
-  CUtensorMap map;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(experts)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_row),
                                  static_cast<cuuint64_t>(stride_expert)};
   const cuuint32_t box[3] = {kBlockKBytes, static_cast<cuuint32_t>(box_rows), 1};
-  const cuuint32_t elem_strides[3] = {1, 1, 1};
-  const CUresult r = encode_tiled_fp8()(
-      &map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box,
-      elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  PPLX_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code " << static_cast<int>(r));
-  return map;
+  return encode_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box);
 }
 
 }  // namespace

@@ -66,20 +66,21 @@
 #include "../core/device_utils.cuh"
 #include "../core/ptx.cuh"
 #include "../core/tcgen05.cuh"
+#include "../core/tensor_map.h"
 #include "../core/utils.h"
 #include "../core/wait.cuh"
 #include "a2a_device.cuh"
 #include "grouped_gemm.h"
+#include "token_cut.cuh"
 #include "token_tile.cuh"
 
 namespace pplx {
 namespace {
 
 using namespace tok;
+using namespace cut;
 
 constexpr int kBlockM = 128;      // weight rows per CTA and tile
-constexpr int kMmaTokens = 256;   // token rows per MMA
-constexpr int kMaxTokens = 512;   // token rows per tile
 constexpr int kBlockK = 64;       // 64 bf16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
 constexpr int kMaxStages = 12;
@@ -111,66 +112,10 @@ struct TokenMaps {
   CUtensorMap x64, x16;
 };
 
-struct Tile {
-  int expert;
-  int w_blk;    // block of weight rows (of the pair or the single CTA)
-  int first;    // first token row of the tile inside its expert
-  int width;    // token rows of the tile, a multiple of kUnit
-  int rows;     // valid rows of the expert
-};
-
-// Token tiles of an expert: as few as `limit` rows per tile allow, as equal as whole units allow.
-template <int kUnit>
-struct Cut {
-  int units, tiles;
-  __device__ __forceinline__ Cut(int rows, int limit)
-      : units((rows + kUnit - 1) / kUnit), tiles((units * kUnit + limit - 1) / limit) {}
-  __device__ __forceinline__ int widest() const { return (units + tiles - 1) / tiles * kUnit; }
-};
-
-template <int kUnit>
-__device__ __forceinline__ Tile locate(const uint32_t* tile_start, const uint32_t* rows_of,
-                                       int num_experts, int limit, uint32_t t) {
-  Tile c;
-  c.expert = find_group(tile_start, num_experts, t);
-  c.rows = static_cast<int>(rows_of[c.expert]);
-  const Cut<kUnit> cut(c.rows, limit);
-  const uint32_t rem = t - tile_start[c.expert];
-  c.w_blk = static_cast<int>(rem / cut.tiles);
-  const int i = static_cast<int>(rem) - c.w_blk * cut.tiles;
-  const int each = cut.units / cut.tiles, wider = cut.units - each * cut.tiles;
-  c.width = (each + (i < wider ? 1 : 0)) * kUnit;
-  c.first = (i * each + min(i, wider)) * kUnit;
-  return c;
-}
-
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b) {
-  return pack_bf16(__uint_as_float(a), __uint_as_float(b));
-}
-
 // Two tokens' results of one column from their gate and up sums.
 __device__ __forceinline__ uint32_t swiglu_pair(uint32_t g0, uint32_t g1, uint32_t u0, uint32_t u1) {
   return pack_bf16(silu(__uint_as_float(g0)) * __uint_as_float(u0),
                    silu(__uint_as_float(g1)) * __uint_as_float(u1));
-}
-
-// Token rows of a tile that its first MMA takes; the second takes the rest.
-__device__ __forceinline__ int first_mma(int width) {
-  return width <= kMmaTokens ? width : ((width >> 1) + 31) & ~31;
-}
-
-template <bool kPair>
-__device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, uint64_t* full, int k,
-                                          int row, int plane) {
-  if constexpr (kPair) tc::tma_load_3d_2cta(dst, map, full, k, row, plane);
-  else tc::tma_load_3d(dst, map, full, k, row, plane);
 }
 
 template <bool SWIGLU, bool kFromStaging, bool kToPeers, bool kPair, bool kWide>
@@ -666,36 +611,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   (void)parity;
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    PPLX_CHECK(q == cudaDriverEntryPointSuccess && p != nullptr,
-               "cuTensorMapEncodeTiled is not available in this driver");
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
-CUtensorMap encode_map(int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-                       const cuuint32_t* box) {
-  PPLX_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "operand base must be 16-byte aligned");
-  const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  CUtensorMap map;
-  const CUresult r = encode_tiled()(
-      &map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box,
-      elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  PPLX_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code " << static_cast<int>(r));
-  return map;
-}
-
 void check_strides(int64_t stride_row_elems, int64_t stride_expert_elems) {
   PPLX_CHECK((stride_row_elems * 2) % 16 == 0 && (stride_expert_elems * 2) % 16 == 0,
              "operand strides must be multiples of 16 bytes (8 bf16 elements)");
@@ -711,7 +626,7 @@ CUtensorMap make_operand_map(const void* base, int64_t planes, int64_t rows, int
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_row_elems) * 2,
                                  static_cast<cuuint64_t>(stride_plane_elems) * 2};
   const cuuint32_t box[3] = {kBlockK, static_cast<cuuint32_t>(box_rows), 1};
-  return encode_map(3, base, dims, strides, box);
+  return encode_map(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box);
 }
 
 // 128 weight rows per tile.  Plain: consecutive ones.  SwiGLU: [experts][2 * n_out][k] seen as
@@ -728,7 +643,7 @@ CUtensorMap make_weight_map(const GroupedGemmCall& c) {
   const cuuint64_t strides[4] = {row, row * static_cast<cuuint64_t>(c.n_out), row * 8,
                                  static_cast<cuuint64_t>(c.w_stride_e) * 2};
   const cuuint32_t box[5] = {kBlockK, 8, 2, 8, 1};
-  return encode_map(5, c.w, dims, strides, box);
+  return encode_map(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, c.w, dims, strides, box);
 }
 
 TokenMaps make_token_maps(const void* base, int64_t planes, int64_t rows, int64_t k,
