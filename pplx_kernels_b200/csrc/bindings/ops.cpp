@@ -1022,6 +1022,7 @@ TORCH_LIBRARY(pplx_kernels_b200, m) {
   pplx::register_all_to_all_ops(m);
   pplx::register_symmetric_memory_ops(m);
   pplx::register_extension_ops(m);
+  pplx::register_expert_ops(m);
 }
 
 PPLX_REGISTER_EXTENSION(libpplx_kernels_b200)

@@ -16,6 +16,8 @@ void register_symmetric_memory_ops(torch::Library& m);
 // Operators beyond the reference's surface: block quantisation, grouped GEMM,
 // fused MoE layer.
 void register_extension_ops(torch::Library& m);
+// Experts of one GPU: tokens sorted by expert and back, products of 8-bit integers.
+void register_expert_ops(torch::Library& m);
 
 }  // namespace pplx
 

@@ -264,6 +264,16 @@ __host__ __device__ constexpr uint32_t make_instr_desc(uint32_t ab_format, int m
          | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// The same for kind::i8: signed 8-bit operands, 32-bit integer sums (they wrap, they do not
+// saturate).
+__host__ __device__ constexpr uint32_t make_instr_desc_i8(int m, int n) {
+  return (2u << 4)                              // accumulator format: s32
+         | (1u << 7)                            // A: signed
+         | (1u << 10)                           // B: signed
+         | (static_cast<uint32_t>(n >> 3) << 17)
+         | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
 // ---- hardware block scaling (kind::mxf8f6f4.block_scale) ----
 //
 // Every 32 K-elements of a row of A and of a column of B carry one power-of-two scale (E8M0:
@@ -337,6 +347,19 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t tmem_d, uint64_t desc_a, uint
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_i8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                          uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
       "}\n"
       :
       : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)

@@ -122,3 +122,37 @@ void launch_gemm_fp8_from_staging(const Fp8GemmCall& call, const A2AParams& p,
 void launch_gemm_fp8_to_peers(const Fp8GemmCall& call, const A2AParams& p, cudaStream_t stream);
 
 }  // namespace pplx
+
+namespace pplx {
+
+// Grouped GEMM of 8-bit integers with one fp32 scale per token row and per weight row.  Payload
+// strides in bytes (= elements), scale strides in floats; the innermost strides are 1.
+struct Int8GemmCall {
+  const void* x = nullptr;       // s8 [E][rows_per_expert][k], or with offsets [rows_per_expert][k]
+  int64_t x_stride_e = 0, x_stride_row = 0;
+  const float* sx = nullptr;     // [E][rows_per_expert], or [rows_per_expert]
+  int64_t sx_stride_e = 0;
+  const void* w = nullptr;       // s8 [E][n_out or 2 * n_out][k]
+  int64_t w_stride_e = 0, w_stride_row = 0;
+  const float* sw = nullptr;     // [E][n_out or 2 * n_out]
+  int64_t sw_stride_e = 0;
+  const int32_t* counts = nullptr;   // [E] rows of each expert; null: all rows of its plane
+  const int32_t* offsets = nullptr;  // [E] first row of each expert, all in one plane; x_stride_e,
+                                     // sx_stride_e and out_stride_e are 0 then
+  void* out = nullptr;           // bf16 or fp16 [E][rows_per_expert][n_out], or [rows_per_expert][n_out]
+  int64_t out_stride_e = 0, out_stride_row = 0;  // elements
+  uint32_t* status = nullptr;    // optional device word, set to 1 if a wait ran out
+  int num_experts = 0;
+  int rows_per_expert = 0;       // rows of a plane
+  int n_out = 0, k = 0;
+  bool swiglu = false;           // w = [gate; up]; the result is silu(gate) * up
+  bool fp16 = false;             // the type of out
+  int64_t expected_total_rows = 0;  // hint for the choice of the kernel form; 0 = capacity
+};
+
+// Throws for sizes and alignments that the kernel does not take.
+void check_grouped_gemm_int8(const Int8GemmCall& call);
+// Rows beyond an expert's count are untouched.
+void launch_grouped_gemm_int8(const Int8GemmCall& call, cudaStream_t stream);
+
+}  // namespace pplx

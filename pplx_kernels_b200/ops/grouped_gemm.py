@@ -127,3 +127,56 @@ def grouped_gemm_fp8_reference(xq: torch.Tensor, sa: torch.Tensor, wq: torch.Ten
             y = torch.nn.functional.silu(y[:, :n_out]) * y[:, n_out:]
         out[e, :m] = y
     return out
+
+
+def grouped_gemm_int8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
+                      w_scale: torch.Tensor, counts: torch.Tensor | None = None,
+                      offsets: torch.Tensor | None = None, swiglu: bool = False,
+                      out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                      status: torch.Tensor | None = None, expected_rows: int = 0) -> torch.Tensor:
+    """Grouped GEMM of 8-bit integers (tcgen05 ``kind::i8``), a scale per token and per channel.
+
+    ``wq`` [E, N (or 2N), K] int8 with ``w_scale`` [E, N (or 2N)] fp32, one per row of ``wq``
+    (``quantize_rows_int8`` of the weights).  The tokens' rows in one of two layouts:
+
+    * ``xq`` [E, rows, K] int8, ``x_scale`` [E, rows] fp32, ``counts`` [E] int32 valid rows per
+      expert (None: all of them; a plain product of two matrices is E = 1 without counts) -> out
+      [E, rows, N];
+    * ``xq`` [rows, K], ``x_scale`` [rows], with ``counts`` and ``offsets``, the number of rows and
+      the first row of every expert (``sort_by_expert``) -> out [rows, N].
+
+    ``out[r] = x_scale[r] * w_scale[e] * (xq[r] @ wq[e].T)``, the sums exact in 32-bit integers
+    (K at most 131071, a multiple of 16); with ``swiglu``, ``wq`` stacks gate and up rows and the
+    result is ``silu(gate) * up``.  ``out`` is bf16 or fp16 (``out_dtype`` where it is allocated
+    here), rounded once.  Rows without a token are left untouched.  ``status`` (int32, optional) is
+    set to 1 if a wait ran out.  ``expected_rows`` (total valid rows, 0 = capacity) is a hint for
+    the choice of the kernel form.
+    """
+    n_out = wq.size(1) // 2 if swiglu else wq.size(1)
+    if out is None:
+        out = torch.empty(*xq.shape[:-1], n_out, dtype=out_dtype, device=xq.device)
+    _ops.grouped_gemm_int8(xq, x_scale, wq, w_scale, counts, offsets, out, swiglu, status,
+                           expected_rows)
+    return out
+
+
+def grouped_gemm_int8_reference(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
+                                w_scale: torch.Tensor, counts: torch.Tensor | None = None,
+                                offsets: torch.Tensor | None = None,
+                                swiglu: bool = False) -> torch.Tensor:
+    """Plain PyTorch fp64 statement of the same operation (rows without a token are zero)."""
+    f64 = torch.float64
+    n_out = wq.size(1) // 2 if swiglu else wq.size(1)
+    out = torch.zeros(*xq.shape[:-1], n_out, dtype=f64, device=xq.device)
+    for e in range(wq.size(0)):
+        m = xq.size(-2) if counts is None else int(counts[e])
+        if offsets is not None:
+            mine: tuple | slice = slice(int(offsets[e]), int(offsets[e]) + m)
+        else:
+            mine = (e, slice(0, m))
+        y = xq[mine].to(f64) @ wq[e].to(f64).t()
+        y = y * x_scale[mine].to(f64)[:, None] * w_scale[e].to(f64)[None, :]
+        if swiglu:
+            y = torch.nn.functional.silu(y[:, :n_out]) * y[:, n_out:]
+        out[mine] = y
+    return out

@@ -1,5 +1,6 @@
-"""Block-scaled fp8 (e4m3) quantisation in plain PyTorch: the oracle for the
-quantisation that ``AllToAll.dispatch_quant`` fuses into the send.
+"""Quantisation: block-scaled fp8 (e4m3) in plain PyTorch, the oracle for what
+``AllToAll.dispatch_quant`` fuses into the send, and rows of 8-bit integers, the input of
+``grouped_gemm_int8``.
 
 One fp32 scale per ``block`` (128) consecutive columns of a row:
 ``scale = max(amax, 1e-4) / 448`` and ``q = round_to_e4m3(x * (448 / max(amax, 1e-4)))``.
@@ -8,6 +9,8 @@ One fp32 scale per ``block`` (128) consecutive columns of a row:
 from __future__ import annotations
 
 import torch
+
+from . import _ops
 
 
 def per_token_block_quant(x: torch.Tensor, block: int = 128,
@@ -37,3 +40,35 @@ def block_dequant(q: torch.Tensor, scale: torch.Tensor, block: int = 128) -> tor
     hidden = q.size(-1)
     s = scale.repeat_interleave(block, dim=-1)[..., :hidden]
     return q.to(torch.float32) * s
+
+
+def quantize_rows_int8(x: torch.Tensor, counts: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None, out_scale: torch.Tensor | None = None,
+                       ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of 8-bit integers with one fp32 scale each: ``x ~= q * scale``.
+
+    ``x`` [rows, k] or [experts, rows, k] in bf16, fp16 or fp32 (weights, one row per channel, or
+    activations).  With ``a = max(max |x|, 1e-30)`` of a row, ``scale = a / 127`` and ``q =
+    round(x * (127 / a))``, ties to even, in fp32, within [-127, 127].  A row with an
+    infinity or a NaN gets that as its scale and zeros in place of the value, so that what is
+    computed with the row is not finite either.  ``counts`` [experts] int32, with x of [experts,
+    rows, k]: rows at or beyond an expert's count are left as they are.
+    """
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("quantize_rows_int8: no gradient is recorded here; use torch.no_grad() or detach()")
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    if out_scale is None:
+        out_scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _ops.quantize_rows_int8(x, counts, out, out_scale)
+    return out, out_scale
+
+
+def quantize_rows_int8_reference(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Plain PyTorch statement of ``quantize_rows_int8`` for finite rows."""
+    v = x.to(torch.float32)
+    amax = v.abs().amax(dim=-1).clamp(min=1e-30)
+    # (A quotient of two tensors is one; with a number torch multiplies by a rounded reciprocal.)
+    most = torch.full_like(amax, 127.0)
+    q = torch.round(v * (most / amax).unsqueeze(-1)).clamp(-127, 127).to(torch.int8)
+    return q, amax / most
