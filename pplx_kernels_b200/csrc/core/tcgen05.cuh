@@ -187,6 +187,14 @@ __device__ __forceinline__ void mbar_arrive_on_leader(uint64_t* bar) {
                : "memory");
 }
 
+// The same for a thread that has nothing to publish but that its tensor-memory loads are over
+// (tcgen05.wait::ld): a release would also wait for its stores to global memory, about 1400 cycles.
+__device__ __forceinline__ void mbar_arrive_on_leader_relaxed(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                   smem_u32(bar) & kPeerBitMask)
+               : "memory");
+}
+
 // -------------------------------------------------------- tensor memory ----
 
 // Whole-warp calls.  `ncols` is a power of two in [32, 512].
@@ -381,6 +389,19 @@ __device__ __forceinline__ void mma_f16_ss_2cta(uint32_t tmem_d, uint64_t desc_a
       : "memory");
 }
 
+__device__ __forceinline__ void mma_i8_ss_2cta(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                               uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
 // Arrival on the mbarrier at this offset in every CTA of `cta_mask` once the pair's
 // MMAs issued so far have finished.  (Multicast of a barrier arrival, not of data.)
 __device__ __forceinline__ void mma_commit_2cta(uint64_t* bar, uint16_t cta_mask) {
@@ -396,6 +417,23 @@ __device__ __forceinline__ void mma_commit_2cta(uint64_t* bar, uint16_t cta_mask
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    smem_u32(bar))
+               : "memory");
+}
+
+// 16 lanes x 32 columns as four blocks of eight columns: thread t receives columns 2 * (t % 4) and
+// the next one of lane t / 4 (r[4 * b], r[4 * b + 1]) and of lane t / 4 + 8 (r[4 * b + 2], r[4 * b + 3]).
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// The same wait as below, for loads into `r`: what uses them cannot be moved in front of it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
                : "memory");
 }
 

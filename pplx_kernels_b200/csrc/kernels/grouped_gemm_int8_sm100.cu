@@ -11,11 +11,20 @@
 // As in the bf16 kernel the WEIGHTS are the M operand of the MMAs and the tokens the N operand, so
 // the work follows the rows there are; a stage of 128 bytes of K holds 128 integers, twice what a
 // stage of the bf16 kernel holds.  A CTA owns a tile of 128 weight rows times a token tile of 16
-// to 256 rows of one expert.
+// to 256 rows of one expert; or a CTA pair (cta_group::2) 256 weight rows, 128 in each CTA, times 32
+// to 512, of which each CTA loads half (above 256 as two MMAs that share the weights).  No TMA
+// multicast is involved.
 //
-// Roles (persistent over tiles): warp 0 TMA producer, warp 1 MMA issuer, warp 2 tensor-memory
-// allocation, warps 4-11 epilogue.  Two accumulators of 256 columns let the epilogue of a tile run
-// under the MMAs of the next.  Every mbarrier wait is bounded: when one runs out the CTA raises a
+// What bounds it, at 6.5 TB/s of HBM and 3.36 POPS (twice the bf16 rate): the weights' bytes up to
+// some 128 rows per expert (32 experts of 2048 x 7168, up projection, 64 rows each: 144 us, floor 147
+// with the rows), L2 around 256 rows (175 us, floor 158), the tensor cores and the power limit above
+// (1024 rows: 600 us = 3.2 POPS; 8 experts of 4096 x 14336, down, 1024 rows: 296 us).  An epilogue that
+// divided by the IEEE quotient and met two barriers per 16 tokens bound the tiles with short K: 128
+// experts of 768 x 2048, up, 256 rows 191 us, now 92; down 77 -> 68.
+//
+// Roles (persistent over tiles): warp 0 TMA producer, warp 1 MMA issuer (leader CTA only), warp 2
+// tensor-memory allocation, warps 4-11 epilogue.  Two accumulators of 256 columns let the epilogue
+// of a tile run under the MMAs of the next; wider tiles have one of 512.  Every mbarrier wait is bounded: when one runs out the CTA raises a
 // shared abort flag, all roles leave their loops, in-flight TMA loads are drained, tensor memory is
 // freed and the kernel returns with *status = 1.
 #include <algorithm>
@@ -45,13 +54,13 @@ constexpr int kBlockK = 128;      // integers = bytes: one 128-byte swizzle row
 constexpr int kUmmaK = 32;
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 384;
-constexpr int kTmemCols = 512;    // two accumulators of 256 columns
+constexpr int kTmemCols = 512;    // an accumulator of kMaxTokens columns, or two of half of them
 constexpr uint32_t kRowBytes = kBlockK;
 constexpr uint32_t kWBytes = kBlockM * kRowBytes;
 constexpr uint32_t kWaitLimitNs = 2000000000u;  // 2 s per wait
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 131071;
-constexpr int kSegBytes = 256 + 16;  // 128 columns of 16 bits of one token, padded
+constexpr int kDrain = 22;        // cycles per token row to read out an accumulator that is the only one
 
 struct Int8GemmArgs {
   const int32_t* counts;   // [num_experts] valid rows per expert; null: rows_per_expert
@@ -80,8 +89,8 @@ struct Control {
   uint32_t max_rows;
   uint32_t max_width;
   unsigned long long best_limit;
+  alignas(128) uint8_t seg[8][32 * 64];  // of each epilogue warp: 32 tokens' columns
   alignas(16) float sx[2][kMaxTokens];  // scales of a tile's tokens, of two tiles in turn
-  alignas(16) uint8_t seg[2][2][16][kSegBytes];  // [warp group][alternating][token][column]
 };
 
 struct TokenMaps {
@@ -92,19 +101,27 @@ __device__ __forceinline__ float scaled(uint32_t sum, float sx, float sw) {
   return static_cast<float>(static_cast<int32_t>(sum)) * sx * sw;
 }
 
+// silu(gate) * up; the quotient by the hardware's reciprocal (2 steps of fp32 off).
+__device__ __forceinline__ float swiglu(float gate, float up) {
+  return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+}
+
 __device__ __forceinline__ uint32_t pack(float a, float b, bool fp16) {
   if (!fp16) return pack_bf16(a, b);
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <bool SWIGLU>
+template <bool SWIGLU, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w,
                              const __grid_constant__ TokenMaps tmap_x,
                              const __grid_constant__ Int8GemmArgs g) {
-  constexpr int kUnit = 16;
+  constexpr int kCtas = kPair ? 2 : 1;
+  constexpr int kUnit = 16 * kCtas;  // steps of an MMA's N: 16, or 32 for M = 256 over a pair
   constexpr int kCols = SWIGLU ? kBlockM / 2 : kBlockM;  // output columns per CTA and tile
+  constexpr int kWarpCols = kCols / 4;       // of an epilogue warp
+  constexpr int kPieces = kWarpCols / 8;     // 16-byte pieces of a token's row in them
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -113,10 +130,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* rows_of = tile_start + g.num_experts + 1;           // [E] valid rows
   uint32_t* row0_of = rows_of + g.num_experts;                  // [E] first row in the token plane
 
-  const uint32_t worker = blockIdx.x, workers = gridDim.x;
+  const uint32_t cta_rank = kPair ? tc::cluster_ctarank() : 0u;
+  const bool leader = cta_rank == 0u;
+  const uint32_t worker = blockIdx.x / kCtas;   // tile-loop index
+  const uint32_t workers = gridDim.x / kCtas;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
-  const int w_blocks = ceil_div<int>(g.n_out, kCols);
+  const int w_blocks = ceil_div<int>(g.n_out, kCols * kCtas);
   const int num_kb = ceil_div<int>(g.k, kBlockK);
 
   // ---- set-up ---------------------------------------------------------------
@@ -124,13 +144,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     ctl->abort_flag = 0;
     ctl->max_rows = 0;
     ctl->max_width = kUnit;
+    ctl->best_limit = ~0ull;
     for (int s = 0; s < kMaxStages; ++s) {
       tc::mbar_init(&ctl->full[s], 1);
       tc::mbar_init(&ctl->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(&ctl->tmem_full[b], 1);
-      tc::mbar_init(&ctl->tmem_empty[b], 8);  // epilogue warps
+      tc::mbar_init(&ctl->tmem_empty[b], 8 * kCtas);  // epilogue warps of the tile
     }
     tc::fence_mbar_init();
     tc::tma_prefetch_desc(&tmap_w);
@@ -138,13 +159,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::tma_prefetch_desc(&tmap_x.x16);
   }
   if (warp == 2) {
-    tc::tmem_alloc(&ctl->tmem_base, kTmemCols);
-    tc::tmem_relinquish();
+    if constexpr (kPair) {
+      tc::tmem_alloc_2cta(&ctl->tmem_base, kTmemCols);
+      tc::tmem_relinquish_2cta();
+    } else {
+      tc::tmem_alloc(&ctl->tmem_base, kTmemCols);
+      tc::tmem_relinquish();
+    }
   }
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   __syncthreads();
-  constexpr int limit = kMmaTokens;
   for (int e = tid; e < g.num_experts; e += blockDim.x) {
     // (Counts and offsets that do not fit the tensors are cut to them.)
     int first = 0, most = g.rows_per_expert;
@@ -155,7 +180,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows = g.counts != nullptr ? min(max(g.counts[e], 0), most) : most;
     rows_of[e] = static_cast<uint32_t>(rows);
     row0_of[e] = static_cast<uint32_t>(first);
-    const Cut<kUnit> cut(rows, limit);
+    if (rows > 0) atomicMax(&ctl->max_rows, static_cast<uint32_t>(rows));
+  }
+  __syncthreads();
+  // The most token rows a tile may have.  One tile per expert up to 256 rows: there an expert is
+  // bound by its weights, which more tiles would only read again.  Above, the limit that
+  // minimises (waves of tiles) x (time of a tile).  A tile of w rows was measured to take 330 + 5/3 w
+  // cycles per K block of 128 bytes up to 256 rows and 220 + 11/5 w above (fewer stages): more than
+  // the 2 w cycles of its MMAs, because L2 delivers some 42 bytes per cycle and SM, of 16 KB of
+  // weights and 64 w bytes of tokens.  More than 256 rows leave no second accumulator, so their
+  // epilogue is not hidden.  Every CTA computes the same.  (32 experts of 2048 x 7168, up projection,
+  // 320 rows each: one tile of 320 213 us, two of 160 246 us; 384: 244, 274 us; 512: 312, 313 us.)
+  int limit = kPair ? kMaxTokens : kMmaTokens;
+  if (ctl->max_rows > kMmaTokens) {
+    for (int cand = limit - kUnit * warp; 4 * cand >= limit; cand -= kUnit * (kThreads / 32)) {
+      uint32_t tiles = 0, width = 0;
+      for (int e = lane; e < g.num_experts; e += 32) {
+        const Cut<kUnit> cut(static_cast<int>(rows_of[e]), cand);
+        tiles += cut.tiles;
+        width += cut.units * kUnit;
+      }
+      tiles = __reduce_add_sync(0xffffffffu, tiles);
+      width = __reduce_add_sync(0xffffffffu, width);
+      if (lane == 0) {
+        const uint64_t waves = ceil_div<uint64_t>(static_cast<uint64_t>(tiles) * w_blocks, workers);
+        const uint32_t w = width / tiles;
+        const uint64_t each = max(330u + 5u * w / 3u, 220u + 11u * w / 5u);
+        const uint64_t cost = waves * (num_kb * each + (cand > kMmaTokens ? kDrain * w : 0u));
+        atomicMin(&ctl->best_limit, (cost << 16) | static_cast<uint64_t>(kMaxTokens - cand));
+      }
+    }
+    __syncthreads();
+    limit = kMaxTokens - static_cast<int>(ctl->best_limit & 0xffffu);
+  }
+  for (int e = tid; e < g.num_experts; e += blockDim.x) {
+    const Cut<kUnit> cut(static_cast<int>(rows_of[e]), limit);
     tile_start[e] = static_cast<uint32_t>(cut.tiles * w_blocks);
     if (cut.tiles > 0) atomicMax(&ctl->max_width, static_cast<uint32_t>(cut.widest()));
   }
@@ -163,12 +222,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) warp_exclusive_scan_smem(tile_start, g.num_experts, lane, true);
   tc::tc_fence_before_sync();
   __syncthreads();
+  // The peer must see initialised barriers before anything arrives on them remotely.
+  if constexpr (kPair) tc::cluster_sync();
   tc::tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
   const uint32_t total_tiles = tile_start[g.num_experts];
   // As many stages as the launch's widest token tile leaves room for.
-  const uint32_t stage_bytes = kWBytes + ctl->max_width * kRowBytes;
+  const uint32_t stage_bytes = kWBytes + ctl->max_width / kCtas * kRowBytes;
   const uint32_t stages = min(g.ring_bytes / stage_bytes, static_cast<uint32_t>(kMaxStages));
+  const bool two = !kPair || ctl->max_width <= kMmaTokens;  // two accumulators
 
   // ---- roles ----------------------------------------------------------------
   if (warp == 0) {
@@ -179,10 +241,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = *abort_flag == 0u;
       for (uint32_t t = worker; t < total_tiles && ok; t += workers) {
         const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
-        const int row0 = static_cast<int>(row0_of[c.expert]) + c.first;
+        // This CTA's share of the tokens of each MMA.
+        const int n0 = kPair ? first_mma(c.width) : c.width;
+        const int own0 = n0 / kCtas, own1 = (c.width - n0) / kCtas;
+        const int tile_row = static_cast<int>(row0_of[c.expert]) + c.first;
+        const int row0 = tile_row + static_cast<int>(cta_rank) * own0;
+        const int row1 = tile_row + n0 + static_cast<int>(cta_rank) * own1;
         const int x_plane = g.offsets != nullptr ? 0 : c.expert;
-        const int w_row = c.w_blk * kCols;
-        const uint32_t tx = kWBytes + static_cast<uint32_t>(c.width) * kRowBytes;
+        const int w_row = (c.w_blk * kCtas + static_cast<int>(cta_rank)) * kCols;
+        const uint32_t tx = kCtas * kWBytes + static_cast<uint32_t>(c.width) * kRowBytes;
         for (int kb = 0; kb < num_kb; ++kb) {
           ok = tc::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, kWaitLimitNs);
           if (!ok) break;
@@ -191,16 +258,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint64_t* full = &ctl->full[stage];
           pending |= 1u << stage;
           pending_phase = (pending_phase & ~(1u << stage)) | (phase << stage);
-          tc::mbar_arrive_expect_tx(full, tx);
-          if constexpr (SWIGLU)
-            tc::tma_load_5d(w_dst, &tmap_w, full, kb * kBlockK, 0, 0, w_row / 8, c.expert);
-          else
-            load_rows<false>(w_dst, &tmap_w, full, kb * kBlockK, w_row, c.expert);
-          int r = 0;
-          for (; r + 64 <= c.width; r += 64, x_dst += 64 * kRowBytes)
-            load_rows<false>(x_dst, &tmap_x.x64, full, kb * kBlockK, row0 + r, x_plane);
-          for (; r < c.width; r += 16, x_dst += 16 * kRowBytes)
-            load_rows<false>(x_dst, &tmap_x.x16, full, kb * kBlockK, row0 + r, x_plane);
+          // The bytes of both CTAs are counted on the leader's barrier, which only the leader
+          // arms.
+          if (leader) tc::mbar_arrive_expect_tx(full, tx);
+          if constexpr (SWIGLU) {
+            if constexpr (kPair)
+              tc::tma_load_5d_2cta(w_dst, &tmap_w, full, kb * kBlockK, 0, 0, w_row / 8, c.expert);
+            else
+              tc::tma_load_5d(w_dst, &tmap_w, full, kb * kBlockK, 0, 0, w_row / 8, c.expert);
+          } else {
+            load_rows<kPair>(w_dst, &tmap_w, full, kb * kBlockK, w_row, c.expert);
+          }
+          auto load_tokens = [&](int row, int n) {
+            int r = 0;
+            for (; r + 64 <= n; r += 64, x_dst += 64 * kRowBytes)
+              load_rows<kPair>(x_dst, &tmap_x.x64, full, kb * kBlockK, row + r, x_plane);
+            for (; r < n; r += 16, x_dst += 16 * kRowBytes)
+              load_rows<kPair>(x_dst, &tmap_x.x16, full, kb * kBlockK, row + r, x_plane);
+          };
+          load_tokens(row0, own0);
+          if constexpr (kPair) load_tokens(row1, own1);
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
@@ -213,7 +290,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t t0 = ptx::globaltimer_ns();
         for (uint32_t s = 0; s < stages; ++s) {
           if (!((pending >> s) & 1u)) continue;
-          while (!tc::mbar_try_wait(&ctl->full[s], (pending_phase >> s) & 1u)) {
+          // (The non-leader of a pair has no barrier of its own to watch; it just sits
+          // out the time limit, which is far longer than any load takes.)
+          while (!leader || !tc::mbar_try_wait(&ctl->full[s], (pending_phase >> s) & 1u)) {
             if (ptx::globaltimer_ns() - t0 > 100000000ull) break;  // 100 ms in total
           }
         }
@@ -221,14 +300,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (tc::elect_one()) {
+    if (leader && tc::elect_one()) {
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = *abort_flag == 0u;
       for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
         const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
-        const uint32_t idesc = tc::make_instr_desc_i8(kBlockM, c.width);
-        const uint32_t buf = local & 1u;
-        const uint32_t use = local >> 1;  // how often this accumulator was used before
+        const int n0 = kPair ? first_mma(c.width) : c.width, n1 = c.width - n0;
+        const uint32_t idesc = tc::make_instr_desc_i8(kBlockM * kCtas, n0);
+        const uint32_t idesc1 = tc::make_instr_desc_i8(kBlockM * kCtas, n1);
+        const uint32_t buf = two ? local & 1u : 0u;
+        const uint32_t use = two ? local >> 1 : local;  // how often this accumulator was used before
         ok = tc::mbar_wait(&ctl->tmem_empty[buf], (use & 1u) ^ 1u, abort_flag, kWaitLimitNs);
         if (!ok) break;
         tc::tc_fence_after_sync();
@@ -241,31 +322,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t w_desc = tc::make_smem_desc_sw128(w_src);
           const uint64_t x_desc = tc::make_smem_desc_sw128(w_src + kWBytes);
 #pragma unroll
-          for (int k = 0; k < kBlockK / kUmmaK; ++k)
-            tc::mma_i8_ss(tmem_d, tc::advance_smem_desc(w_desc, k * kUmmaK),
-                          tc::advance_smem_desc(x_desc, k * kUmmaK), idesc, (kb | k) != 0);
-          tc::mma_commit(&ctl->empty[stage]);
+          for (int k = 0; k < kBlockK / kUmmaK; ++k) {
+            const uint64_t wd = tc::advance_smem_desc(w_desc, k * kUmmaK);
+            const uint64_t xd = tc::advance_smem_desc(x_desc, k * kUmmaK);
+            if constexpr (kPair) tc::mma_i8_ss_2cta(tmem_d, wd, xd, idesc, (kb | k) != 0);
+            else tc::mma_i8_ss(tmem_d, wd, xd, idesc, (kb | k) != 0);
+          }
+          if constexpr (kPair) {
+            if (n1 > 0) {
+              const uint64_t x1_desc = tc::advance_smem_desc(x_desc, n0 / kCtas * kRowBytes);
+#pragma unroll
+              for (int k = 0; k < kBlockK / kUmmaK; ++k)
+                tc::mma_i8_ss_2cta(tmem_d + n0, tc::advance_smem_desc(w_desc, k * kUmmaK),
+                                   tc::advance_smem_desc(x1_desc, k * kUmmaK), idesc1, (kb | k) != 0);
+            }
+          }
+          // Stage reusable (in both CTAs of a pair) once these MMAs have read it.
+          if constexpr (kPair) tc::mma_commit_2cta(&ctl->empty[stage], 0x3);
+          else tc::mma_commit(&ctl->empty[stage]);
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) tc::mma_commit(&ctl->tmem_full[buf]);
+        if (ok) {
+          if constexpr (kPair) tc::mma_commit_2cta(&ctl->tmem_full[buf], 0x3);
+          else tc::mma_commit(&ctl->tmem_full[buf]);
+        }
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
     const int ew = (warp - 4) & 3;   // tensor-memory lanes [32 * ew, +32)
-    const int wg = (warp - 4) >> 2;  // 16-token groups wg, wg + 2, wg + 4, ...
-    const int n_tid = tid - 128;     // 0..255 over the eight warps
-    const int lt = n_tid & 127;      // thread of the warp group
+    const int wg = (warp - 4) >> 2;  // 32-token groups wg, wg + 2, wg + 4, ...
+    const int n_tid = tid - 128;     // over the epilogue warps
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
     uint32_t local = 0;
     bool ok = *abort_flag == 0u;
     for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
       const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
       const int live = min(c.width, c.rows - c.first);  // tokens of the tile that exist
-      const int col0 = c.w_blk * kCols;
+      const int col0 = (c.w_blk * kCtas + static_cast<int>(cta_rank)) * kCols;
       const int64_t row0 = static_cast<int64_t>(row0_of[c.expert]) + c.first;
       // The tile's scales, while its MMAs run.  (The table of the tile before is still read: the
       // barrier below is what ends that.)
@@ -275,15 +372,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       float sw[4];  // plain: weight rows lane / 4 + 0, 8, 16, 24; SwiGLU: gate, up of two columns
       {
         const float* s = g.sw + c.expert * g.sw_stride_e;
-        const int col = col0 + (SWIGLU ? ew * 16 : ew * 32) + (lane >> 2);
+        const int col = col0 + kWarpCols * ew + (lane >> 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = SWIGLU ? col + (i >> 1) * 8 : col + i * 8;
           sw[i] = at < g.n_out ? s[SWIGLU && (i & 1) ? g.n_out + at : at] : 0.0f;
         }
       }
-      const uint32_t buf = local & 1u;
-      ok = tc::mbar_wait(&ctl->tmem_full[buf], (local >> 1) & 1u, abort_flag, kWaitLimitNs);
+      // Where this thread stores: token lane / kPieces of every 32 / kPieces, 16 bytes.
+      const int store_token = lane / kPieces, store_piece = lane % kPieces;
+      const int store_col = col0 + kWarpCols * ew + store_piece * 8;
+      uint16_t* out = g.out + c.expert * g.out_stride_e + row0 * g.out_stride_row + store_col;
+      const int stored = store_col + 8 <= g.n_out ? live : 0;
+      const uint32_t buf = two ? local & 1u : 0u;
+      ok = tc::mbar_wait(&ctl->tmem_full[buf], (two ? local >> 1 : local) & 1u, abort_flag, kWaitLimitNs);
       // All eight warps leave together or not at all: the barriers below must never be
       // entered by only some of them.
       {
@@ -292,76 +394,103 @@ __global__ void __launch_bounds__(kThreads, 1)
             "{\n\t"
             ".reg .pred p, q;\n\t"
             "setp.ne.u32 q, %1, 0;\n\t"
-            "bar.red.and.pred p, 1, 256, q;\n\t"
+            "bar.red.and.pred p, 1, %2, q;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t"
             "}\n"
             : "=r"(all_ok)
-            : "r"(ok ? 1u : 0u)
+            : "r"(ok ? 1u : 0u), "n"(256)
             : "memory");
         ok = all_ok != 0u;
       }
       if (!ok) break;
       tc::tc_fence_after_sync();
-      const int groups = c.width >> 4;
+      const int groups = (c.width + 31) >> 5;
       const uint32_t t_acc = t_lane + buf * kMmaTokens;
-      // A thread's values lie across token rows; each group of 16 tokens passes through shared
-      // memory so that rows leave in 16-byte pieces.
-#pragma unroll 1
-      for (int grp = wg, alt = 0; grp < groups; grp += 2, alt ^= 1) {
-        uint32_t lo[8], hi[8];
-        load_group(t_acc + grp * 16, lo, hi);
-        const float2 s0 = *reinterpret_cast<const float2*>(&sx[grp * 16 + 2 * (lane & 3)]);
-        const float2 s1 = *reinterpret_cast<const float2*>(&sx[grp * 16 + 8 + 2 * (lane & 3)]);
-        tc::tmem_ld_wait();
-        uint8_t(*seg)[kSegBytes] = ctl->seg[wg][alt];
-        if constexpr (SWIGLU) {
-          // Lanes 0-7 of every 16 are gate rows, 8-15 the up rows of the same columns.
-          auto pair = [&](const uint32_t* v, float2 s, float gate, float up) {
-            return pack(silu(scaled(v[0], s.x, gate)) * scaled(v[2], s.x, up),
-                        silu(scaled(v[1], s.y, gate)) * scaled(v[3], s.y, up), g.fp16);
-          };
-          stmatrix_x4_trans(&seg[8 * (lane >> 4) + (lane & 7)][(ew * 16 + ((lane >> 3) & 1) * 8) * 2],
-                            pair(lo, s0, sw[0], sw[1]), pair(hi, s0, sw[2], sw[3]),
-                            pair(lo + 4, s1, sw[0], sw[1]), pair(hi + 4, s1, sw[2], sw[3]));
-        } else {
+      // The accumulator is handed back when the warp has its last columns in registers.
+      auto hand_back = [&] {
+        tc::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) tc::mbar_arrive_on_leader_relaxed(&ctl->tmem_empty[buf]);
+          else tc::mbar_arrive(&ctl->tmem_empty[buf]);
+        }
+      };
+      // 32 tokens at a time, the next ones on their way while these are finished.  A thread's values
+      // lie across token rows; they pass through shared memory of the warp's own, so that rows leave
+      // in 16-byte pieces.  (The pieces of a row of shared memory are in an order that keeps both
+      // sides free of bank conflicts.)
+      uint8_t* seg = ctl->seg[warp - 4];
+      auto at = [&](int token, int piece) {
+        return seg + token * (kPieces * 16) + ((piece ^ (token / (8 / kPieces) % kPieces)) * 16);
+      };
+      auto finish = [&](int grp, const uint32_t (&lo)[16], const uint32_t (&hi)[16]) {
+        __syncwarp();  // (the tokens before have been read)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float2 s = b == 0 ? s0 : s1;
+        for (int b = 0; b < 4; b += SWIGLU ? 2 : 1) {
+          const float2 s = *reinterpret_cast<const float2*>(&sx[grp * 32 + 8 * b + 2 * (lane & 3)]);
+          if constexpr (SWIGLU) {
+            // Lanes 0-7 of every 16 are gate rows, 8-15 the up rows of the same columns.
+            const float2 s1 = *reinterpret_cast<const float2*>(&sx[grp * 32 + 8 * b + 8 + 2 * (lane & 3)]);
+            auto pair = [&](const uint32_t* v, float2 t, float gate, float up) {
+              return pack(swiglu(scaled(v[0], t.x, gate), scaled(v[2], t.x, up)),
+                          swiglu(scaled(v[1], t.y, gate), scaled(v[3], t.y, up)), g.fp16);
+            };
+            stmatrix_x4_trans(at(8 * b + 8 * (lane >> 4) + (lane & 7), (lane >> 3) & 1),
+                              pair(lo + 4 * b, s, sw[0], sw[1]), pair(hi + 4 * b, s, sw[2], sw[3]),
+                              pair(lo + 4 * b + 4, s1, sw[0], sw[1]),
+                              pair(hi + 4 * b + 4, s1, sw[2], sw[3]));
+          } else {
             auto pair = [&](uint32_t v0, uint32_t v1, float w) {
               return pack(scaled(v0, s.x, w), scaled(v1, s.y, w), g.fp16);
             };
-            stmatrix_x4_trans(&seg[8 * b + (lane & 7)][(ew * 32 + (lane >> 3) * 8) * 2],
-                              pair(lo[4 * b], lo[4 * b + 1], sw[0]),
+            stmatrix_x4_trans(at(8 * b + (lane & 7), lane >> 3), pair(lo[4 * b], lo[4 * b + 1], sw[0]),
                               pair(lo[4 * b + 2], lo[4 * b + 3], sw[1]),
                               pair(hi[4 * b], hi[4 * b + 1], sw[2]),
                               pair(hi[4 * b + 2], hi[4 * b + 3], sw[3]));
           }
         }
-        sync_group(wg);
-        constexpr int kPieces = kCols / 8;  // 16-byte pieces of a token's row segment
-        const int piece = lt % kPieces;
-        const int col = col0 + piece * 8;
+        __syncwarp();
 #pragma unroll
-        for (int tok16 = lt / kPieces; tok16 < 16; tok16 += 128 / kPieces) {
-          const int n = grp * 16 + tok16;
-          const int4 v = *reinterpret_cast<const int4*>(&seg[tok16][piece * 16]);
-          if (n < live && col + 8 <= g.n_out)
-            *reinterpret_cast<int4*>(g.out + c.expert * g.out_stride_e +
-                                     (row0 + n) * g.out_stride_row + col) = v;
+        for (int t0 = 0; t0 < 32; t0 += 32 / kPieces) {
+          const int n = grp * 32 + t0 + store_token;
+          const int4 v = *reinterpret_cast<const int4*>(at(t0 + store_token, store_piece));
+          if (n < stored) *reinterpret_cast<int4*>(out + n * g.out_stride_row) = v;
         }
+      };
+      uint32_t lo[2][16], hi[2][16];
+      int grp = wg;
+      auto load = [&](int which, int from) {
+        tc::tmem_ld_16x256b_x4(t_acc + from * 32, lo[which]);
+        tc::tmem_ld_16x256b_x4(t_acc + (16u << 16) + from * 32, hi[which]);
+      };
+      if (grp < groups) load(0, grp);
+      else hand_back();
+      auto step = [&](int now) {
+        tc::tmem_ld_wait(lo[now]);
+        tc::tmem_ld_wait(hi[now]);
+        if (grp + 2 < groups) load(now ^ 1, grp + 2);
+        else hand_back();
+        finish(grp, lo[now], hi[now]);
+        grp += 2;
+      };
+#pragma unroll 1
+      while (grp < groups) {
+        step(0);
+        if (grp < groups) step(1);
       }
-      tc::tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&ctl->tmem_empty[buf]);
     }
   }
 
   // ---- teardown -------------------------------------------------------------
   tc::tc_fence_before_sync();
   __syncthreads();
+  // Neither CTA of a pair may leave while the other can still touch its shared or
+  // tensor memory.
+  if constexpr (kPair) tc::cluster_sync();
   if (warp == 2) {
     tc::tc_fence_after_sync();
-    tc::tmem_dealloc(tmem_base, kTmemCols);
+    if constexpr (kPair) tc::tmem_dealloc_2cta(tmem_base, kTmemCols);
+    else tc::tmem_dealloc(tmem_base, kTmemCols);
   }
   if (tid == 0 && ctl->abort_flag != 0u && g.status != nullptr) *g.status = 1u;
 }
@@ -393,10 +522,10 @@ CUtensorMap make_weight_map(const Int8GemmCall& c) {
   return encode_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.w, dims, strides, box);
 }
 
-template <bool SWIGLU>
+template <bool SWIGLU, bool kPair>
 void launch_one(const CUtensorMap& tmap_w, const TokenMaps& tmap_x, Int8GemmArgs g, int grid,
                 cudaStream_t stream) {
-  auto* kernel = grouped_gemm_int8_kernel<SWIGLU>;
+  auto* kernel = grouped_gemm_int8_kernel<SWIGLU, kPair>;
   const size_t fixed =
       1024 + sizeof(Control) + sizeof(uint32_t) * (3 * static_cast<size_t>(g.num_experts) + 1);
   // The stages take what the tables leave, at least three of the widest.
@@ -409,8 +538,30 @@ void launch_one(const CUtensorMap& tmap_w, const TokenMaps& tmap_x, Int8GemmArgs
   CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(smem)));
   void* params[] = {const_cast<CUtensorMap*>(&tmap_w), const_cast<TokenMaps*>(&tmap_x), &g};
-  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(grid),
-                                   dim3(kThreads), params, smem, stream, 1));
+  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(kPair ? (grid & ~1) : grid),
+                                   dim3(kThreads), params, smem, stream, kPair ? 2 : 1));
+}
+
+// Single CTAs, whose tiles of 128 weight rows divide a launch more finely, up to an expected mean of
+// 112 rows per expert; pairs, which read the tokens half as often, from there on.  us, single and
+// pairs: 128 experts of 768 x 2048, up projection 2 rows 65.1 / 68.8, 64 rows 70.7 / 76.8, 128 rows
+// 78.0 / 81.1, 256 rows 98.5 / 92.4; 32 experts of 2048 x 7168, up 8 rows 143.0 / 141.4, 128 rows
+// 153.7 / 150.7, 256 rows 198 / 176; down 64 rows 81.0 / 84.3, 128 rows 89.1 / 88.3, 256 rows 116.5 /
+// 104.9.
+bool want_pairs(const Int8GemmCall& c) {
+  const int64_t rows = c.expected_total_rows > 0 ? c.expected_total_rows
+                       : c.offsets != nullptr
+                           ? c.rows_per_expert
+                           : static_cast<int64_t>(c.num_experts) * c.rows_per_expert;
+  return rows > 112 * static_cast<int64_t>(c.num_experts);
+}
+
+template <bool SWIGLU>
+void launch_variant(const CUtensorMap& tmap_w, const TokenMaps& tmap_x, const Int8GemmArgs& g,
+                    const Int8GemmCall& c, cudaStream_t stream) {
+  const int grid = get_sm_count();
+  if (want_pairs(c) && grid >= 2) launch_one<SWIGLU, true>(tmap_w, tmap_x, g, grid, stream);
+  else launch_one<SWIGLU, false>(tmap_w, tmap_x, g, grid, stream);
 }
 
 }  // namespace
@@ -457,9 +608,8 @@ void launch_grouped_gemm_int8(const Int8GemmCall& c, cudaStream_t stream) {
   g.n_out = c.n_out;
   g.k = c.k;
   g.fp16 = c.fp16;
-  const int grid = get_sm_count();
-  if (c.swiglu) launch_one<true>(tmap_w, tmap_x, g, grid, stream);
-  else launch_one<false>(tmap_w, tmap_x, g, grid, stream);
+  if (c.swiglu) launch_variant<true>(tmap_w, tmap_x, g, c, stream);
+  else launch_variant<false>(tmap_w, tmap_x, g, c, stream);
 }
 
 }  // namespace pplx
