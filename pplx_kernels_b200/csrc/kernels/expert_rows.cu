@@ -8,12 +8,14 @@
 #include "expert_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "../core/device_utils.cuh"
 #include "../core/ptx.cuh"
+#include "../core/tcgen05.cuh"
 #include "../core/utils.h"
 
 namespace pplx {
@@ -24,18 +26,29 @@ constexpr int kMaxSortExperts = 1024;
 
 // ------------------------------------------------------------------------ sort ----
 
-constexpr int kSortThreads = 1024;
+constexpr int kSortThreads = 512;
+
+__device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t cta) {
+  uint32_t addr, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tc::smem_u32(p)), "r"(cta));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 // Warps take runs of entries.  A warp counts its entries per expert and remembers for each entry
-// how many of its expert came before it in the run; the runs' counts are then summed over the warps
-// and the experts.
+// how many of its expert came before it in the run; the runs' counts are then summed over the warps,
+// the blocks (one, or a cluster whose blocks read each other's sums) and the experts.  Bound by
+// latency: of the entries' loads, the match of 32 entries, three block barriers.
 template <typename Index>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExpertCall c) {
   extern __shared__ uint32_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const int blocks = gridDim.x;
   const int E = c.num_experts;
   uint32_t* seen = smem;               // [warps][E]
-  uint32_t* first = smem + warps * E;  // [E + 1]
+  uint32_t* mine_all = smem + warps * E;  // [E] entries of this block
+  uint32_t* first = mine_all + E;      // [E + 1]
+  for (int i = tid; i < warps * E; i += blockDim.x) seen[i] = 0;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   const Index* indices = static_cast<const Index*>(c.indices);
@@ -43,10 +56,12 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
   int live = n;
   if (c.bound_m != nullptr)
     live = static_cast<int>(min(*c.bound_m, static_cast<uint32_t>(c.num_tokens))) * c.topk;
-  for (int i = tid; i < warps * E; i += blockDim.x) seen[i] = 0;
   __syncthreads();
-  const int per = (ceil_div(n, warps) + 31) & ~31;
-  const int begin = min(warp * per, n), end = min(begin + per, n);
+  const int runs = warps * blocks;
+  const int per = (ceil_div(n, runs) + 31) & ~31;
+  const int run = blockIdx.x * warps + warp;
+  const int begin = static_cast<int>(min(static_cast<int64_t>(run) * per, static_cast<int64_t>(n)));
+  const int end = min(begin + per, n);
   uint32_t* mine = seen + warp * E;
   for (int i0 = begin; i0 < end; i0 += 32) {
     const int i = i0 + lane;
@@ -65,20 +80,40 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
   }
   __syncthreads();
   for (int e = tid; e < E; e += blockDim.x) {
-    uint32_t run = 0;
+    uint32_t sum = 0;
     for (int w = 0; w < warps; ++w) {
       const uint32_t v = seen[w * E + e];
-      seen[w * E + e] = run;
-      run += v;
+      seen[w * E + e] = sum;
+      sum += v;
     }
-    first[e] = run;
-    c.counts[e] = c.capacity > 0 ? min(static_cast<int>(run), c.capacity) : static_cast<int>(run);
+    mine_all[e] = sum;
+    first[e] = sum;
   }
+  if (blocks > 1) {
+    tc::cluster_sync();
+    for (int e = tid; e < E; e += blockDim.x) {
+      uint32_t sum = 0, before = 0;
+      for (int b = 0; b < blocks; ++b) {
+        const uint32_t v = ld_cluster(&mine_all[e], b);
+        if (b == static_cast<int>(blockIdx.x)) before = sum;
+        sum += v;
+      }
+      first[e] = sum;
+      for (int w = 0; w < warps; ++w) seen[w * E + e] += before;
+    }
+    tc::cluster_sync();  // (no block leaves while others read its sums)
+  } else {
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)
+    for (int e = tid; e < E; e += blockDim.x)
+      c.counts[e] = c.capacity > 0 ? min(static_cast<int>(first[e]), c.capacity) : static_cast<int>(first[e]);
   __syncthreads();
   if (warp == 0) warp_exclusive_scan_smem(first, E, lane, true);
   __syncthreads();
-  for (int e = tid; e <= E; e += blockDim.x)
-    c.offsets[e] = c.capacity > 0 ? e * c.capacity : static_cast<int>(first[e]);
+  if (blockIdx.x == 0)
+    for (int e = tid; e <= E; e += blockDim.x)
+      c.offsets[e] = c.capacity > 0 ? e * c.capacity : static_cast<int>(first[e]);
   for (int i = begin + lane; i < end; i += 32) {
     const int32_t local = c.row_of[i];  // (of this thread)
     if (local < 0) continue;
@@ -104,24 +139,91 @@ __device__ __forceinline__ int row_at(const ExpertRowsView& v, int64_t t, int k)
   return static_cast<uint32_t>(r) < static_cast<uint64_t>(v.num_rows) ? r : -1;
 }
 
-template <typename T, int kVec>
-struct alignas(sizeof(T) * kVec) Pack {
-  T v[kVec];
+// kVec elements of a row as the words that memory moves: registers hold 16-bit values in pairs.
+template <int kBytes>
+struct Words {
+  using type = uint32_t;
+};
+template <>
+struct Words<16> {
+  using type = uint4;
+};
+template <>
+struct Words<8> {
+  using type = uint2;
+};
+template <>
+struct Words<2> {
+  using type = uint16_t;
+};
+template <>
+struct Words<1> {
+  using type = uint8_t;
 };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <>
-__device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
+template <typename T, int kVec>
+struct Vec {
+  static constexpr int kBytes = kVec * static_cast<int>(sizeof(T));
+  static constexpr int kWords = (kBytes + 3) / 4;
+  using Memory = typename Words<kBytes>::type;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void set(const Memory& m) {
+    if constexpr (kBytes == 16) w[0] = m.x, w[1] = m.y, w[2] = m.z, w[3] = m.w;
+    else if constexpr (kBytes == 8) w[0] = m.x, w[1] = m.y;
+    else w[0] = m;
+  }
+  __device__ __forceinline__ void load(const void* row, int col) {
+    set(reinterpret_cast<const Memory*>(row)[col]);
+  }
+  // What is read once leaves no copy in L1.
+  __device__ __forceinline__ void load_once(const void* row, int col) {
+    const Memory* p = reinterpret_cast<const Memory*>(row) + col;
+    if constexpr (kBytes == 16) {
+      const int4 v = ptx::ld_nc_v4(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+      set(*p);
+    }
+  }
+  __device__ __forceinline__ void store(void* row, int col) const {
+    Memory m;
+    if constexpr (kBytes == 16) m = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (kBytes == 8) m = make_uint2(w[0], w[1]);
+    else m = static_cast<Memory>(w[0]);
+    reinterpret_cast<Memory*>(row)[col] = m;
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else if constexpr (std::is_same_v<T, __half>)
+      return __half2float(__ushort_as_half(static_cast<uint16_t>(j & 1 ? w[j >> 1] >> 16 : w[j >> 1])));
+    else return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+  }
+  __device__ __forceinline__ void put(const float (&v)[kVec]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) w[j] = __float_as_uint(v[j]);
+    } else if constexpr (kVec == 1) {
+      if constexpr (std::is_same_v<T, __half>) w[0] = __half_as_ushort(__float2half_rn(v[0]));
+      else w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; j += 2) {
+        if constexpr (std::is_same_v<T, __half>) {
+          const __half2 h = __floats2half2_rn(v[j], v[j + 1]);
+          w[j >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[j], v[j + 1]);
+          w[j >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+    }
+  }
+};
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
@@ -171,8 +273,8 @@ __global__ void __launch_bounds__(kThreads) permute_kernel(const PermuteCall c) 
 // A warp per (token, piece of 32 vectors).
 template <typename T, int kVec>
 __global__ void __launch_bounds__(kThreads) unpermute_kernel(const UnpermuteCall c) {
-  constexpr int kBatch = 4;  // rows whose vectors a lane has in flight
-  using P = Pack<T, kVec>;
+  constexpr int kBatch = 8;  // rows whose vectors a lane has in flight
+  using V = Vec<T, kVec>;
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
@@ -185,78 +287,102 @@ __global__ void __launch_bounds__(kThreads) unpermute_kernel(const UnpermuteCall
        u < tokens * pieces; u += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t t = u / pieces;
     const int col = static_cast<int>(u - t * pieces) * 32 + lane;
-    if (col >= vecs) continue;
     float sum[kVec] = {};
     for (int k0 = 0; k0 < r.topk; k0 += kBatch) {
-      P v[kBatch];
-      float w[kBatch];
+      // Lane k holds entry k0 + k.
+      int my_row = -1;
+      float my_w = 0.0f;
+      if (lane < kBatch && k0 + lane < r.topk) {
+        my_row = row_at(r, t, k0 + lane);
+        my_w = my_row < 0 ? 0.0f : c.weights != nullptr ? c.weights[t * r.topk + k0 + lane] : 1.0f;
+      }
+      V v[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int row = k0 + b < r.topk ? row_at(r, t, k0 + b) : -1;
-        w[b] = row < 0 ? 0.0f : c.weights != nullptr ? c.weights[t * r.topk + k0 + b] : 1.0f;
-        v[b] = P{};
-        if (row >= 0)
-          v[b] = reinterpret_cast<const P*>(static_cast<const T*>(c.y) +
-                                            static_cast<int64_t>(row) * c.hidden)[col];
+        const int row = __shfl_sync(kAll, my_row, b);
+        v[b].clear();
+        if (row >= 0 && col < vecs)
+          v[b].load_once(static_cast<const T*>(c.y) + static_cast<int64_t>(row) * c.hidden, col);
       }
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
+      for (int b = 0; b < kBatch; ++b) {
+        const float w = __shfl_sync(kAll, my_w, b);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) sum[j] = fmaf(w[b], to_float(v[b].v[j]), sum[j]);
+        for (int j = 0; j < kVec; ++j) sum[j] = fmaf(w, v[b].get(j), sum[j]);
+      }
     }
-    P o;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) o.v[j] = from_float<T>(sum[j]);
-    reinterpret_cast<P*>(static_cast<T*>(c.out) + t * c.out_stride)[col] = o;
+    if (col >= vecs) continue;
+    V o;
+    o.put(sum);
+    o.store(static_cast<T*>(c.out) + t * c.out_stride, col);
   }
 }
 
 // A block per token; behind the tokens, a block per row to be cleared.
 template <typename T, int kVec>
 __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const UnpermuteBackwardCall c) {
-  constexpr int kBatch = 4;
-  using P = Pack<T, kVec>;
+  constexpr int kBatch = 8;
+  using V = Vec<T, kVec>;
   __shared__ float part[kBatch][kWarps];
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   const int vecs = c.hidden / kVec;
   auto row_ptr = [&](auto* base, int64_t row) { return base + row * c.hidden; };
   const int64_t blocks = r.num_tokens + (c.grad_y != nullptr ? r.num_rows : 0);
   for (int64_t t = blockIdx.x; t < blocks; t += gridDim.x) {
     if (t >= r.num_tokens) {
       const int64_t row = t - r.num_tokens;
+      V zero;
+      zero.clear();
       if (is_rest(r, row))
-        for (int col = tid; col < vecs; col += kThreads)
-          reinterpret_cast<P*>(row_ptr(static_cast<T*>(c.grad_y), row))[col] = P{};
+        for (int col = tid; col < vecs; col += threads)
+          zero.store(row_ptr(static_cast<T*>(c.grad_y), row), col);
       continue;
     }
-    const P* grad = reinterpret_cast<const P*>(static_cast<const T*>(c.grad) + t * c.grad_stride);
+    const T* grad = static_cast<const T*>(c.grad) + t * c.grad_stride;
     for (int k0 = 0; k0 < r.topk; k0 += kBatch) {
-      int row[kBatch];
-      float w[kBatch], dot[kBatch] = {};
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        row[b] = k0 + b < r.topk ? row_at(r, t, k0 + b) : -1;
-        w[b] = k0 + b < r.topk ? c.weights[t * r.topk + k0 + b] : 0.0f;
+      // Lane k holds entry k0 + k.
+      int my_row = -1;
+      float my_w = 0.0f;
+      if (lane < kBatch && k0 + lane < r.topk) {
+        my_row = row_at(r, t, k0 + lane);
+        my_w = c.weights[t * r.topk + k0 + lane];
       }
-      for (int col = tid; col < vecs; col += kThreads) {
-        const P g = grad[col];
+      float dot[kBatch] = {};
+      for (int col0 = 0; col0 < vecs; col0 += threads) {
+        const int col = col0 + tid;
+        const bool in = col < vecs;
+        V g, y[kBatch];
+        g.clear();
+        if (in) g.load(grad, col);
+        if (c.grad_weights != nullptr) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          if (row[b] < 0) continue;
-          if (c.grad_weights != nullptr) {
-            const P y = reinterpret_cast<const P*>(row_ptr(static_cast<const T*>(c.y), row[b]))[col];
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) dot[b] = fmaf(to_float(y.v[j]), to_float(g.v[j]), dot[b]);
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = __shfl_sync(kAll, my_row, b);
+            y[b].clear();
+            if (row >= 0 && in) y[b].load_once(row_ptr(static_cast<const T*>(c.y), row), col);
           }
-          if (c.grad_y != nullptr) {
-            P o;
+        }
+        if (c.grad_y != nullptr) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) o.v[j] = from_float<T>(w[b] * to_float(g.v[j]));
-            reinterpret_cast<P*>(row_ptr(static_cast<T*>(c.grad_y), row[b]))[col] = o;
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = __shfl_sync(kAll, my_row, b);
+            const float w = __shfl_sync(kAll, my_w, b);
+            float v[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[j] = w * g.get(j);
+            V o;
+            o.put(v);
+            if (row >= 0 && in) o.store(row_ptr(static_cast<T*>(c.grad_y), row), col);
           }
+        }
+        if (c.grad_weights != nullptr) {
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) dot[b] = fmaf(y[b].get(j), g.get(j), dot[b]);
         }
       }
       if (c.grad_weights == nullptr) continue;
@@ -270,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const Unpe
       __syncthreads();
       if (tid < kBatch && k0 + tid < r.topk) {
         float s = 0.0f;
-        for (int w2 = 0; w2 < kWarps; ++w2) s += part[tid][w2];
+        for (int w2 = 0; w2 < threads / 32; ++w2) s += part[tid][w2];
         c.grad_weights[t * r.topk + k0 + tid] = s;
       }
       __syncthreads();
@@ -290,66 +416,120 @@ __device__ __forceinline__ float row_amax(uint32_t bits) {
   return __uint_as_float(max(bits, __float_as_uint(1e-30f)));
 }
 
-__device__ __forceinline__ int8_t quantize(float v, float inv) {
-  return static_cast<int8_t>(max(min(__float2int_rn(v * inv), 127), -127));
+// rint(v * inv) of four values, |v * inv| <= 127.0001, as bytes: adding 1.5 * 2^23 rounds to whole
+// numbers, which are then the low bits.  (The product is rounded before: no fused add.)
+__device__ __forceinline__ uint32_t quantize(float a, float b, float c, float d, float inv) {
+  auto whole = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f)); };
+  return __byte_perm(__byte_perm(whole(a), whole(b), 0x0040), __byte_perm(whole(c), whole(d), 0x0040),
+                     0x5410);
 }
 
-// A block per token (or row of x); behind them, a block per row to be cleared.
-template <typename T, int kVec>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeRowsCall c,
-                                                            const ExpertRowsView r) {
-  using P = Pack<T, kVec>;
-  using Q = Pack<int8_t, kVec>;
-  __shared__ uint32_t part[kWarps];
+// A team of threads per token (or row of x): a warp (kWarpTeam), or the block; behind them, a team
+// per row to be cleared.  The first kHeld vectors of a thread stay in registers between the search
+// for the largest value and the rounding; longer rows are read again for the rest.
+template <typename T, int kVec, int kHeld, bool kWarpTeam, bool kPermuted>
+__global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
+    quantize_kernel(const QuantizeRowsCall c, const ExpertRowsView r) {
+  using V = Vec<T, kVec>;
+  using Q = Vec<int8_t, kVec>;
+  __shared__ uint32_t part[2][kWarps];
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = kWarpTeam ? lane : threadIdx.x, threads = kWarpTeam ? 32 : blockDim.x;
+  const int teams = kWarpTeam ? blockDim.x >> 5 : 1;
   const int vecs = c.hidden / kVec;
-  const bool permuted = r.row_of != nullptr;
-  const int64_t sources = permuted ? r.num_tokens : c.num_rows;
-  const int64_t blocks = sources + (c.zero_rest ? r.num_rows : 0);
-  for (int64_t t = blockIdx.x; t < blocks; t += gridDim.x) {
+  const int64_t sources = kPermuted ? r.num_tokens : c.num_rows;
+  const int64_t items = sources + (c.zero_rest ? r.num_rows : 0);
+  int turn = 0;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * teams + (kWarpTeam ? warp : 0); t < items;
+       t += static_cast<int64_t>(gridDim.x) * teams) {
     if (t >= sources) {
       const int64_t row = t - sources;
       if (!is_rest(r, row)) continue;
-      for (int col = tid; col < vecs; col += kThreads)
-        reinterpret_cast<Q*>(c.q + row * c.hidden)[col] = Q{};
+      Q zero;
+      zero.clear();
+      for (int col = tid; col < vecs; col += threads) zero.store(c.q + row * c.hidden, col);
       if (tid == 0) c.scale[row] = 0.0f;
       continue;
     }
-    if (c.counts != nullptr) {
+    if (!kPermuted && c.counts != nullptr) {
       const int64_t plane = t / c.plane_rows;
       if (t - plane * c.plane_rows >= c.counts[plane]) continue;
     }
-    const P* x = reinterpret_cast<const P*>(static_cast<const T*>(c.x) + t * c.x_stride);
-    uint32_t bits = 0;
-    for (int col = tid; col < vecs; col += kThreads) {
-      const P v = x[col];
+    const T* x = static_cast<const T*>(c.x) + t * c.x_stride;
+    V held[kHeld];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) bits = max(bits, magnitude(to_float(v.v[j])));
+    for (int h = 0; h < kHeld; ++h) {
+      const int col = tid + h * threads;
+      held[h].clear();
+      if (col < vecs) held[h].load_once(x, col);
+    }
+    int my_row = -1;  // lane k holds that of entry k
+    if (kPermuted && lane < r.topk) my_row = row_at(r, t, lane);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) bits = max(bits, magnitude(held[h].get(j)));
+#pragma unroll 1
+    for (int col = tid + kHeld * threads; col < vecs; col += threads) {
+      V v;
+      v.load(x, col);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) bits = max(bits, magnitude(v.get(j)));
     }
     bits = __reduce_max_sync(kAll, bits);
-    if (lane == 0) part[warp] = bits;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) bits = max(bits, part[w]);
-    __syncthreads();
+    if constexpr (!kWarpTeam) {
+      if (lane == 0) part[turn][warp] = bits;
+      __syncthreads();
+      bits = __reduce_max_sync(kAll, lane < threads / 32 ? part[turn][lane] : 0u);
+      turn ^= 1;  // (the next row's maxima go elsewhere, so one barrier is enough)
+    }
     const float amax = row_amax(bits);
     const float inv = 127.0f / amax, scale = amax / 127.0f;
-    const int targets = permuted ? r.topk : 1;
-    for (int col = tid; col < vecs; col += kThreads) {
-      const P v = x[col];
+    // A row with an infinity or a NaN is zero throughout.
+    const uint32_t keep = amax < __uint_as_float(0x7f800000u) ? 0xffffffffu : 0u;
+    auto rounded = [&](const V& v) {
       Q o;
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) o.v[j] = quantize(to_float(v.v[j]), inv);
+      for (int j = 0; j < kVec; j += 4)
+        o.w[j >> 2] = keep & quantize(v.get(j), kVec > 1 ? v.get(min(j + 1, kVec - 1)) : 0.0f,
+                                      kVec > 2 ? v.get(min(j + 2, kVec - 1)) : 0.0f,
+                                      kVec > 2 ? v.get(min(j + 3, kVec - 1)) : 0.0f, inv);
+      return o;
+    };
+    const int targets = kPermuted ? r.topk : 1;
+    auto row_to = [&](int k) -> int64_t {
+      if constexpr (!kPermuted) return t;
+      return k < 32 ? __shfl_sync(kAll, my_row, k) : row_at(r, t, k);
+    };
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      const int col = tid + h * threads;
+      const Q q = rounded(held[h]);
+#pragma unroll 1
       for (int k = 0; k < targets; ++k) {
-        const int64_t row = permuted ? row_at(r, t, k) : t;
-        if (row >= 0) reinterpret_cast<Q*>(c.q + row * c.hidden)[col] = o;
+        const int64_t row = row_to(k);
+        if (row >= 0 && col < vecs) q.store(c.q + row * c.hidden, col);
       }
     }
-    for (int k = tid; k < targets; k += kThreads) {
-      const int64_t row = permuted ? row_at(r, t, k) : t;
-      if (row >= 0) c.scale[row] = scale;
+#pragma unroll 1
+    for (int col0 = kHeld * threads; col0 < vecs; col0 += threads) {
+      const int col = col0 + tid;
+      V v;
+      v.clear();
+      if (col < vecs) v.load(x, col);
+      const Q q = rounded(v);
+#pragma unroll 1
+      for (int k = 0; k < targets; ++k) {
+        const int64_t row = row_to(k);
+        if (row >= 0 && col < vecs) q.store(c.q + row * c.hidden, col);
+      }
+    }
+    for (int k = 0; k < targets; ++k) {
+      const int64_t row = row_to(k);
+      if (row >= 0 && tid == 0) c.scale[row] = scale;
     }
   }
 }
@@ -366,16 +546,17 @@ int alignment(int most, std::initializer_list<uint64_t> values) {
 uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Enough blocks to fill every SM with 2048 threads; they loop over the rest.
-unsigned blocks_for(int64_t wanted) {
-  return static_cast<unsigned>(
-      std::max<int64_t>(1, std::min<int64_t>(wanted, static_cast<int64_t>(get_sm_count()) * 8)));
+unsigned blocks_for(int64_t wanted, int threads) {
+  const int64_t most = static_cast<int64_t>(get_sm_count()) * std::min(32, 2048 / threads);
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(wanted, most)));
 }
 
 template <typename Call>
-void launch(void (*kernel)(const Call), const Call& c, int64_t blocks, cudaStream_t stream) {
+void launch(void (*kernel)(const Call), const Call& c, int64_t blocks, cudaStream_t stream,
+            int threads = kThreads) {
   void* params[] = {const_cast<Call*>(&c)};
-  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(blocks_for(blocks)),
-                                   dim3(kThreads), params, 0, stream));
+  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel),
+                                   dim3(blocks_for(blocks, threads)), dim3(threads), params, 0, stream));
 }
 
 // Calls fn(T{}, integral_constant<kVec>) for the type and for vectors of `bytes` bytes.
@@ -402,13 +583,21 @@ int size_of(FloatType t) { return t == FloatType::kFloat ? 4 : 2; }
 void launch_sort_by_expert(const SortByExpertCall& c, cudaStream_t stream) {
   PPLX_CHECK(c.num_experts > 0 && c.num_experts <= kMaxSortExperts, "num_experts out of range");
   auto* kernel = c.wide_indices ? sort_kernel<uint64_t> : sort_kernel<uint32_t>;
-  const int warps = kSortThreads / 32;
-  const size_t smem = sizeof(uint32_t) * (static_cast<size_t>(warps + 1) * c.num_experts + 1);
+  const int64_t n = static_cast<int64_t>(c.num_tokens) * c.topk;
+  // us with 256 experts, one block of 256 / 512 threads, clusters of 8 / 16 blocks of 512: 8 entries
+  // 2.8 / 3.0 / 4.7 / 5.3, 512 entries 3.9 / 3.7 / 5.2 / 5.9, 1024 entries 4.6 / 4.5 / 5.3 / 5.8, 4096
+  // entries 10.0 / 7.9 / 5.4 / 5.9, 8192 entries 17.0 / 12.9 / 6.1 / 5.9, 32768 entries 80 / 51 /
+  // 10.7 / 8.1.
+  const int blocks = n <= 1024 ? 1 : n <= 8192 ? 8 : 16;
+  const int threads = n <= 256 ? 256 : kSortThreads;
+  const int warps = threads / 32;
+  const size_t smem = sizeof(uint32_t) * (static_cast<size_t>(warps + 2) * c.num_experts + 1);
   CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(smem)));
+  CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   void* params[] = {const_cast<SortByExpertCall*>(&c)};
-  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(1),
-                                   dim3(kSortThreads), params, smem, stream));
+  CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(blocks), dim3(threads),
+                                   params, smem, stream, static_cast<unsigned>(blocks)));
 }
 
 void launch_permute_tokens(const PermuteCall& c, cudaStream_t stream) {
@@ -445,26 +634,45 @@ void launch_unpermute_backward(const UnpermuteBackwardCall& c, cudaStream_t stre
   const int vec = alignment(16, {address(c.y), address(c.grad), address(c.grad_y), c.hidden * size,
                                  c.grad_stride * size});
   with_type(c.type, vec, [&](auto t, auto v) {
-    launch(unpermute_backward_kernel<decltype(t), v.value>, c, blocks, stream);
+    // As few threads as cover a token's vectors in whole turns of the block.
+    const int vecs = c.hidden / v.value;
+    const int turns = std::max(1, ceil_div(vecs, kThreads));
+    const int threads = std::min(kThreads, std::max(32, round_up(ceil_div(vecs, turns), 32)));
+    launch(unpermute_backward_kernel<decltype(t), v.value>, c, blocks, stream, threads);
   });
 }
 
 void launch_quantize_rows(const QuantizeRowsCall& c, cudaStream_t stream) {
   ExpertRowsView r{};
   if (c.rows != nullptr) r = *c.rows;
-  const int64_t blocks = (c.rows != nullptr ? r.num_tokens : c.num_rows) +
-                         (c.zero_rest ? r.num_rows : 0);
-  if (blocks == 0) return;
+  const int64_t items = (c.rows != nullptr ? r.num_tokens : c.num_rows) +
+                        (c.zero_rest ? r.num_rows : 0);
+  if (items == 0) return;
   const uint64_t size = size_of(c.type);
   // A vector of x of `vec` bytes becomes one of vec / size bytes of q.
   const int vec = std::min<int>(
       alignment(16, {address(c.x), c.hidden * size, c.x_stride * size}),
       alignment(16, {address(c.q), static_cast<uint64_t>(c.hidden)}) * static_cast<int>(size));
   with_type(c.type, vec, [&](auto t, auto v) {
-    auto* kernel = quantize_kernel<decltype(t), v.value>;
-    void* params[] = {const_cast<QuantizeRowsCall*>(&c), &r};
-    CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(blocks_for(blocks)),
-                                     dim3(kThreads), params, 0, stream));
+    using T = decltype(t);
+    const int vecs = c.hidden / v.value;
+    auto run = [&](auto* kernel, int threads, int64_t teams_wanted) {
+      void* params[] = {const_cast<QuantizeRowsCall*>(&c), &r};
+      CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel),
+                                       dim3(blocks_for(teams_wanted, threads)), dim3(threads), params,
+                                       0, stream));
+    };
+    auto pick = [&](auto permuted) {
+      constexpr bool kPermuted = decltype(permuted)::value;
+      if (vecs <= 32 * 4)
+        return run(quantize_kernel<T, v.value, 4, true, kPermuted>, kThreads, ceil_div<int64_t>(items, kWarps));
+      if (vecs <= kThreads * 4)
+        return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32), items);
+      const int threads = std::min(kThreads, round_up(ceil_div(vecs, 8), 32));
+      run(quantize_kernel<T, v.value, 8, false, kPermuted>, threads, items);
+    };
+    if (c.rows != nullptr) pick(std::true_type{});
+    else pick(std::false_type{});
   });
 }
 
