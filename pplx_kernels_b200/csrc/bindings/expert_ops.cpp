@@ -1,5 +1,6 @@
 // Operators of the experts of one GPU: tokens sorted by expert and back, with gradients, rows
 // quantised to 8-bit integers, and their grouped GEMM.  No counterpart in the reference.
+#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -131,9 +132,9 @@ const float* weights_ptr(const at::Tensor& weights, const ExpertRowsView& v, con
 
 // ------------------------------------------------------------------------ sort ----
 
-void sort_by_expert_op(const at::Tensor& indices, int64_t num_experts, int64_t capacity,
-                       const std::optional<at::Tensor>& bound_m, at::Tensor& counts,
-                       at::Tensor& offsets, at::Tensor& row_of) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_by_expert_op(
+    const at::Tensor& indices, int64_t num_experts, int64_t capacity,
+    const std::optional<at::Tensor>& bound_m) {
   const char* op = "sort_by_expert";
   check_device(indices, op, "indices");
   TORCH_CHECK(indices.scalar_type() == at::kInt || indices.scalar_type() == at::kUInt32 ||
@@ -142,26 +143,42 @@ void sort_by_expert_op(const at::Tensor& indices, int64_t num_experts, int64_t c
   TORCH_CHECK(indices.dim() == 2 && indices.size(1) > 0 && indices.is_contiguous(), op,
               ": indices must be contiguous, [tokens, topk]");
   TORCH_CHECK(num_experts > 0 && num_experts <= 1024, op, ": num_experts must be in [1, 1024]");
+  TORCH_CHECK(capacity >= 0, op, ": capacity must not be negative");
+  TORCH_CHECK(indices.numel() <= kMaxRows && capacity <= kMaxRows &&
+                  num_experts * capacity <= kMaxRows,
+              op, ": more than 2^30 rows");
+  const uint32_t* bound = bound_ptr(bound_m, indices, op);
+  const auto options = indices.options().dtype(at::kInt);
+  at::Tensor counts = at::empty({num_experts}, options);
+  at::Tensor offsets = at::empty({num_experts + 1}, options);
+  at::Tensor row_of = at::empty(indices.sizes(), options);
   SortByExpertCall c;
-  const ExpertRowsView v = make_view(counts, offsets, row_of, capacity, indices, op);
-  TORCH_CHECK(v.num_experts == num_experts && row_of.sizes() == indices.sizes(), op,
-              ": the results must be [experts], [experts + 1] and [tokens, topk]");
   c.indices = data<void>(indices);
   c.wide_indices = indices.scalar_type() == at::kLong;
-  c.bound_m = bound_ptr(bound_m, indices, op);
-  c.num_tokens = v.num_tokens;
-  c.topk = v.topk;
-  c.num_experts = v.num_experts;
-  c.capacity = v.capacity;
+  c.bound_m = bound;
+  c.num_tokens = static_cast<int>(indices.size(0));
+  c.topk = static_cast<int>(indices.size(1));
+  c.num_experts = static_cast<int>(num_experts);
+  c.capacity = static_cast<int>(capacity);
   c.counts = data<int32_t>(counts);
   c.offsets = data<int32_t>(offsets);
   c.row_of = data<int32_t>(row_of);
   launch_on(indices, [&](cudaStream_t stream) { launch_sort_by_expert(c, stream); });
+  return {counts, offsets, row_of};
 }
 
 // --------------------------------------------------------------------- permute ----
 
-void permute_tokens_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
+at::Tensor empty_rows(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& row_of,
+                      int64_t capacity, at::ScalarType type) {
+  TORCH_CHECK(x.dim() == 2 && counts.dim() == 1 && capacity >= 0 && capacity <= kMaxRows,
+              "tokens must be [tokens, hidden], counts [experts] and capacity not negative");
+  const auto options = x.options().dtype(type);
+  if (capacity > 0) return at::empty({counts.size(0), capacity, x.size(1)}, options);
+  return at::empty({row_of.numel(), x.size(1)}, options);
+}
+
+void permute_tokens_out_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
                        const at::Tensor& row_of, int64_t capacity, at::Tensor& out,
                        bool zero_rest) {
   const char* op = "permute_tokens";
@@ -179,11 +196,18 @@ void permute_tokens_op(const at::Tensor& x, const at::Tensor& counts, const at::
   launch_on(x, [&](cudaStream_t stream) { launch_permute_tokens(c, stream); });
 }
 
+at::Tensor permute_tokens_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
+                             const at::Tensor& row_of, int64_t capacity, bool zero_rest) {
+  at::Tensor out = empty_rows(x, counts, row_of, capacity, x.scalar_type());
+  permute_tokens_out_op(x, counts, offsets, row_of, capacity, out, zero_rest);
+  return out;
+}
+
 void check_hidden(int64_t hidden, const char* op) {
   TORCH_CHECK(hidden < (int64_t{1} << 30), op, ": rows of 2^30 elements or more");
 }
 
-void permute_tokens_int8_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
+void permute_tokens_int8_out_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
                             const at::Tensor& row_of, int64_t capacity, at::Tensor& out,
                             at::Tensor& out_scale, bool zero_rest) {
   const char* op = "permute_tokens_int8";
@@ -209,9 +233,18 @@ void permute_tokens_int8_op(const at::Tensor& x, const at::Tensor& counts, const
   launch_on(x, [&](cudaStream_t stream) { launch_quantize_rows(c, stream); });
 }
 
+std::tuple<at::Tensor, at::Tensor> permute_tokens_int8_op(
+    const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
+    const at::Tensor& row_of, int64_t capacity, bool zero_rest) {
+  at::Tensor out = empty_rows(x, counts, row_of, capacity, at::kChar);
+  at::Tensor scale = at::empty(out.sizes().slice(0, out.dim() - 1), x.options().dtype(at::kFloat));
+  permute_tokens_int8_out_op(x, counts, offsets, row_of, capacity, out, scale, zero_rest);
+  return {out, scale};
+}
+
 // ------------------------------------------------------------------- unpermute ----
 
-void unpermute_tokens_op(const at::Tensor& y, const at::Tensor& counts, const at::Tensor& offsets,
+void unpermute_tokens_out_op(const at::Tensor& y, const at::Tensor& counts, const at::Tensor& offsets,
                          const at::Tensor& row_of, int64_t capacity,
                          const std::optional<at::Tensor>& weights, at::Tensor& out,
                          const std::optional<at::Tensor>& bound_m) {
@@ -232,6 +265,15 @@ void unpermute_tokens_op(const at::Tensor& y, const at::Tensor& counts, const at
   c.out = data<void>(out);
   c.hidden = static_cast<int>(out.size(1));
   launch_on(y, [&](cudaStream_t stream) { launch_unpermute_tokens(c, stream); });
+}
+
+at::Tensor unpermute_tokens_op(const at::Tensor& y, const at::Tensor& counts,
+                               const at::Tensor& offsets, const at::Tensor& row_of,
+                               int64_t capacity, const std::optional<at::Tensor>& weights) {
+  TORCH_CHECK(y.dim() >= 1 && row_of.dim() == 2, "unpermute_tokens: y must be rows, row_of [tokens, topk]");
+  at::Tensor out = at::empty({row_of.size(0), y.size(-1)}, y.options());
+  unpermute_tokens_out_op(y, counts, offsets, row_of, capacity, weights, out, std::nullopt);
+  return out;
 }
 
 void unpermute_tokens_backward_op(const at::Tensor& grad, const at::Tensor& y,
@@ -272,7 +314,7 @@ void unpermute_tokens_backward_op(const at::Tensor& grad, const at::Tensor& y,
 
 // -------------------------------------------------------------------- int8 ----
 
-void quantize_rows_int8_op(const at::Tensor& x, const std::optional<at::Tensor>& counts,
+void quantize_rows_int8_out_op(const at::Tensor& x, const std::optional<at::Tensor>& counts,
                            at::Tensor& out, at::Tensor& out_scale) {
   const char* op = "quantize_rows_int8";
   check_device(x, op, "x");
@@ -310,6 +352,16 @@ void quantize_rows_int8_op(const at::Tensor& x, const std::optional<at::Tensor>&
   c.scale = data<float>(out_scale);
   c.hidden = static_cast<int>(k);
   launch_on(x, [&](cudaStream_t stream) { launch_quantize_rows(c, stream); });
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows_int8_op(const at::Tensor& x,
+                                                         const std::optional<at::Tensor>& counts) {
+  TORCH_CHECK(x.dim() == 2 || x.dim() == 3,
+              "quantize_rows_int8: x must be [rows, k] or [experts, rows, k]");
+  at::Tensor out = at::empty(x.sizes(), x.options().dtype(at::kChar));
+  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  quantize_rows_int8_out_op(x, counts, out, scale);
+  return {out, scale};
 }
 
 // Stride of a dimension; one that is never used counts as `packed`.
@@ -410,29 +462,44 @@ void grouped_gemm_int8_op(const at::Tensor& xq, const at::Tensor& x_scale, const
 }  // namespace
 
 void register_expert_ops(torch::Library& m) {
-  m.def("sort_by_expert(Tensor indices, int num_experts, int capacity, Tensor? bound_m, "
-        "Tensor! counts, Tensor! offsets, Tensor! row_of) -> ()");
+  m.def("sort_by_expert(Tensor indices, int num_experts, int capacity, Tensor? bound_m) -> "
+        "(Tensor counts, Tensor offsets, Tensor row_of)");
   m.impl("sort_by_expert", c10::kCUDA, &sort_by_expert_op);
   m.impl("sort_by_expert", c10::kMeta, &sort_by_expert_op);
   m.def("permute_tokens(Tensor x, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
-        "Tensor! out, bool zero_rest) -> ()");
+        "bool zero_rest) -> Tensor");
   m.impl("permute_tokens", c10::kCUDA, &permute_tokens_op);
   m.impl("permute_tokens", c10::kMeta, &permute_tokens_op);
+  m.def("permute_tokens_out(Tensor x, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
+        "Tensor! out, bool zero_rest) -> ()");
+  m.impl("permute_tokens_out", c10::kCUDA, &permute_tokens_out_op);
+  m.impl("permute_tokens_out", c10::kMeta, &permute_tokens_out_op);
   m.def("permute_tokens_int8(Tensor x, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
-        "Tensor! out, Tensor! out_scale, bool zero_rest) -> ()");
+        "bool zero_rest) -> (Tensor out, Tensor out_scale)");
   m.impl("permute_tokens_int8", c10::kCUDA, &permute_tokens_int8_op);
   m.impl("permute_tokens_int8", c10::kMeta, &permute_tokens_int8_op);
+  m.def("permute_tokens_int8_out(Tensor x, Tensor counts, Tensor offsets, Tensor row_of, "
+        "int capacity, Tensor! out, Tensor! out_scale, bool zero_rest) -> ()");
+  m.impl("permute_tokens_int8_out", c10::kCUDA, &permute_tokens_int8_out_op);
+  m.impl("permute_tokens_int8_out", c10::kMeta, &permute_tokens_int8_out_op);
   m.def("unpermute_tokens(Tensor y, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
-        "Tensor? weights, Tensor! out, Tensor? bound_m) -> ()");
+        "Tensor? weights) -> Tensor");
   m.impl("unpermute_tokens", c10::kCUDA, &unpermute_tokens_op);
   m.impl("unpermute_tokens", c10::kMeta, &unpermute_tokens_op);
+  m.def("unpermute_tokens_out(Tensor y, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
+        "Tensor? weights, Tensor! out, Tensor? bound_m) -> ()");
+  m.impl("unpermute_tokens_out", c10::kCUDA, &unpermute_tokens_out_op);
+  m.impl("unpermute_tokens_out", c10::kMeta, &unpermute_tokens_out_op);
   m.def("unpermute_tokens_backward(Tensor grad, Tensor y, Tensor counts, Tensor offsets, "
         "Tensor row_of, int capacity, Tensor weights, Tensor!? grad_y, Tensor!? grad_weights) -> ()");
   m.impl("unpermute_tokens_backward", c10::kCUDA, &unpermute_tokens_backward_op);
   m.impl("unpermute_tokens_backward", c10::kMeta, &unpermute_tokens_backward_op);
-  m.def("quantize_rows_int8(Tensor x, Tensor? counts, Tensor! out, Tensor! out_scale) -> ()");
+  m.def("quantize_rows_int8(Tensor x, Tensor? counts) -> (Tensor out, Tensor out_scale)");
   m.impl("quantize_rows_int8", c10::kCUDA, &quantize_rows_int8_op);
   m.impl("quantize_rows_int8", c10::kMeta, &quantize_rows_int8_op);
+  m.def("quantize_rows_int8_out(Tensor x, Tensor? counts, Tensor! out, Tensor! out_scale) -> ()");
+  m.impl("quantize_rows_int8_out", c10::kCUDA, &quantize_rows_int8_out_op);
+  m.impl("quantize_rows_int8_out", c10::kMeta, &quantize_rows_int8_out_op);
   m.def("grouped_gemm_int8(Tensor xq, Tensor x_scale, Tensor wq, Tensor w_scale, Tensor? counts, "
         "Tensor? offsets, Tensor! out, bool swiglu, Tensor!? status, int expected_rows=0) -> ()");
   m.impl("grouped_gemm_int8", c10::kCUDA, &grouped_gemm_int8_op);

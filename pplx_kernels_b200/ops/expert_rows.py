@@ -60,25 +60,16 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, capacity: int = 0,
     GPU).  A token may name an expert twice: it then has two of its rows.  ``bound_m`` (32-bit, on
     the device): tokens at or beyond it get no rows.
     """
-    m, topk = indices.shape
-    dev = indices.device
-    # (One allocation for the three results.)
-    buf = torch.empty(m * topk + 2 * num_experts + 1, dtype=torch.int32, device=dev)
-    row_of, counts, offsets = buf.split((m * topk, num_experts, num_experts + 1))
-    row_of = row_of.view(m, topk)
-    _ops.sort_by_expert(indices, num_experts, capacity, bound_m, counts, offsets, row_of)
+    counts, offsets, row_of = _ops.sort_by_expert(indices, num_experts, capacity, bound_m)
     return ExpertRows(counts, offsets, row_of, capacity, bound_m)
 
 
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, counts, offsets, row_of, capacity):
-        rows = ExpertRows(counts, offsets, row_of, capacity)
         ctx.save_for_backward(counts, offsets, row_of)
         ctx.capacity = capacity
-        out = torch.empty(*rows.shape(), x.size(1), dtype=x.dtype, device=x.device)
-        _ops.permute_tokens(x, counts, offsets, row_of, capacity, out, True)
-        return out
+        return _ops.permute_tokens(x, counts, offsets, row_of, capacity, True)
 
     @staticmethod
     @once_differentiable
@@ -96,23 +87,23 @@ def permute_tokens(x: torch.Tensor, rows: ExpertRows, zero_rest: bool | None = N
     set to zero with ``zero_rest``; where a gradient is recorded (``x`` requires one) they are zero,
     and the gradient of ``x[t]`` is the sum of its rows' (in fp32, rounded once; bf16, fp16 and fp32).
     """
-    if out is None and torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         if zero_rest is False:
             raise ValueError("permute_tokens: rows without a token are zero where a gradient is recorded")
+        if out is not None:
+            raise _no_gradient("permute_tokens")
         return _Permute.apply(x, rows.counts, rows.offsets, rows.row_of, rows.capacity)
-    _no_gradient("permute_tokens", x)
     if out is None:
-        out = torch.empty(*rows.shape(), x.size(1), dtype=x.dtype, device=x.device)
-    _ops.permute_tokens(x, rows.counts, rows.offsets, rows.row_of, rows.capacity, out,
-                        bool(zero_rest))
+        return _ops.permute_tokens(x, rows.counts, rows.offsets, rows.row_of, rows.capacity,
+                                   bool(zero_rest))
+    _ops.permute_tokens_out(x, rows.counts, rows.offsets, rows.row_of, rows.capacity, out,
+                            bool(zero_rest))
     return out
 
 
 def permute_tokens_backward(grad: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
     """The gradient of ``permute_tokens`` with respect to the tokens, for that of its result."""
-    out = torch.empty(rows.row_of.size(0), grad.size(-1), dtype=grad.dtype, device=grad.device)
-    _ops.unpermute_tokens(grad, rows.counts, rows.offsets, rows.row_of, rows.capacity, None, out, None)
-    return out
+    return _ops.unpermute_tokens(grad, rows.counts, rows.offsets, rows.row_of, rows.capacity, None)
 
 
 def permute_tokens_int8(x: torch.Tensor, rows: ExpertRows, zero_rest: bool = False,
@@ -120,25 +111,26 @@ def permute_tokens_int8(x: torch.Tensor, rows: ExpertRows, zero_rest: bool = Fal
                         ) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantises every token of ``x`` (bf16, fp16 or fp32) as ``quantize_rows_int8`` does and copies
     it to its rows.  Returns the rows and their fp32 scales.  Not differentiable."""
-    _no_gradient("permute_tokens_int8", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _no_gradient("permute_tokens_int8")
+    if out is None and out_scale is None:
+        return _ops.permute_tokens_int8(x, rows.counts, rows.offsets, rows.row_of, rows.capacity,
+                                        zero_rest)
     if out is None:
         out = torch.empty(*rows.shape(), x.size(1), dtype=torch.int8, device=x.device)
     if out_scale is None:
         out_scale = torch.empty(rows.shape(), dtype=torch.float32, device=x.device)
-    _ops.permute_tokens_int8(x, rows.counts, rows.offsets, rows.row_of, rows.capacity, out, out_scale,
-                             zero_rest)
+    _ops.permute_tokens_int8_out(x, rows.counts, rows.offsets, rows.row_of, rows.capacity, out,
+                                 out_scale, zero_rest)
     return out, out_scale
 
 
 class _Unpermute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, counts, offsets, row_of, capacity):
-        rows = ExpertRows(counts, offsets, row_of, capacity)
         ctx.save_for_backward(y, weights, counts, offsets, row_of)
         ctx.capacity = capacity
-        out = torch.empty(row_of.size(0), y.size(-1), dtype=y.dtype, device=y.device)
-        _ops.unpermute_tokens(y, counts, offsets, row_of, rows.capacity, weights, out, None)
-        return out
+        return _ops.unpermute_tokens(y, counts, offsets, row_of, capacity, weights)
 
     @staticmethod
     @once_differentiable
@@ -162,18 +154,16 @@ def unpermute_tokens(y: torch.Tensor, rows: ExpertRows, weights: torch.Tensor | 
 
     Differentiable in ``y`` and ``weights``; the gradient of rows without a token is zero.
     """
-    if torch.is_grad_enabled() and out is None and (
-            y.requires_grad or (weights is not None and weights.requires_grad)):
+    if (y.requires_grad or (weights is not None and weights.requires_grad)) and torch.is_grad_enabled():
+        if out is not None:
+            raise _no_gradient("unpermute_tokens")
         if weights is None:
             weights = torch.ones(rows.row_of.shape, dtype=torch.float32, device=y.device)
         return _Unpermute.apply(y, weights, rows.counts, rows.offsets, rows.row_of, rows.capacity)
-    _no_gradient("unpermute_tokens", y, weights)
-    bound = None
     if out is None:
-        out = torch.empty(rows.row_of.size(0), y.size(-1), dtype=y.dtype, device=y.device)
-    else:
-        bound = rows.bound_m
-    _ops.unpermute_tokens(y, rows.counts, rows.offsets, rows.row_of, rows.capacity, weights, out, bound)
+        return _ops.unpermute_tokens(y, rows.counts, rows.offsets, rows.row_of, rows.capacity, weights)
+    _ops.unpermute_tokens_out(y, rows.counts, rows.offsets, rows.row_of, rows.capacity, weights, out,
+                              rows.bound_m)
     return out
 
 
@@ -190,10 +180,9 @@ def unpermute_tokens_backward(
     return grad_y, grad_weights
 
 
-def _no_gradient(name: str, *tensors: torch.Tensor | None) -> None:
-    """Refuses a call whose result could not carry the gradient that was asked for."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name}: no gradient is recorded here; use torch.no_grad() or detach()")
+def _no_gradient(name: str) -> ValueError:
+    """The refusal of a call whose result could not carry the gradient that was asked for."""
+    return ValueError(f"{name}: no gradient is recorded here; use torch.no_grad() or detach()")
 
 
 def sort_by_expert_reference(indices: torch.Tensor, num_experts: int, capacity: int = 0,

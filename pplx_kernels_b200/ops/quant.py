@@ -54,13 +54,15 @@ def quantize_rows_int8(x: torch.Tensor, counts: torch.Tensor | None = None,
     computed with the row is not finite either.  ``counts`` [experts] int32, with x of [experts,
     rows, k]: rows at or beyond an expert's count are left as they are.
     """
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("quantize_rows_int8: no gradient is recorded here; use torch.no_grad() or detach()")
+    if out is None and out_scale is None:
+        return _ops.quantize_rows_int8(x, counts)
     if out is None:
         out = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     if out_scale is None:
         out_scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _ops.quantize_rows_int8(x, counts, out, out_scale)
+    _ops.quantize_rows_int8_out(x, counts, out, out_scale)
     return out, out_scale
 
 
