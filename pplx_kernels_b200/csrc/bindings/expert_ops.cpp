@@ -2,7 +2,9 @@
 // quantised to 8-bit integers, and their grouped GEMM.  No counterpart in the reference.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "../core/utils.h"
@@ -36,6 +38,12 @@ void check_device(const at::Tensor& t, const char* op, const char* name) {
 void check_device(const at::Tensor& t, const at::Tensor& like, const char* op, const char* name) {
   TORCH_CHECK(t.device() == like.device(), op, ": ", name, " must be on ", like.device(), ", not on ",
               t.device());
+}
+
+// (For CUDA tensors the allocation itself, without another pass through the dispatcher.)
+at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
+  if (like.is_cuda()) return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+  return at::empty(sizes, like.options().dtype(type));
 }
 
 template <typename T>
@@ -148,10 +156,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_by_expert_op(
                   num_experts * capacity <= kMaxRows,
               op, ": more than 2^30 rows");
   const uint32_t* bound = bound_ptr(bound_m, indices, op);
-  const auto options = indices.options().dtype(at::kInt);
-  at::Tensor counts = at::empty({num_experts}, options);
-  at::Tensor offsets = at::empty({num_experts + 1}, options);
-  at::Tensor row_of = at::empty(indices.sizes(), options);
+  at::Tensor counts = empty({num_experts}, indices, at::kInt);
+  at::Tensor offsets = empty({num_experts + 1}, indices, at::kInt);
+  at::Tensor row_of = empty(indices.sizes(), indices, at::kInt);
   SortByExpertCall c;
   c.indices = data<void>(indices);
   c.wide_indices = indices.scalar_type() == at::kLong;
@@ -173,9 +180,8 @@ at::Tensor empty_rows(const at::Tensor& x, const at::Tensor& counts, const at::T
                       int64_t capacity, at::ScalarType type) {
   TORCH_CHECK(x.dim() == 2 && counts.dim() == 1 && capacity >= 0 && capacity <= kMaxRows,
               "tokens must be [tokens, hidden], counts [experts] and capacity not negative");
-  const auto options = x.options().dtype(type);
-  if (capacity > 0) return at::empty({counts.size(0), capacity, x.size(1)}, options);
-  return at::empty({row_of.numel(), x.size(1)}, options);
+  if (capacity > 0) return empty({counts.size(0), capacity, x.size(1)}, x, type);
+  return empty({row_of.numel(), x.size(1)}, x, type);
 }
 
 void permute_tokens_out_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
@@ -237,7 +243,7 @@ std::tuple<at::Tensor, at::Tensor> permute_tokens_int8_op(
     const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
     const at::Tensor& row_of, int64_t capacity, bool zero_rest) {
   at::Tensor out = empty_rows(x, counts, row_of, capacity, at::kChar);
-  at::Tensor scale = at::empty(out.sizes().slice(0, out.dim() - 1), x.options().dtype(at::kFloat));
+  at::Tensor scale = empty(out.sizes().slice(0, out.dim() - 1), x, at::kFloat);
   permute_tokens_int8_out_op(x, counts, offsets, row_of, capacity, out, scale, zero_rest);
   return {out, scale};
 }
@@ -271,7 +277,7 @@ at::Tensor unpermute_tokens_op(const at::Tensor& y, const at::Tensor& counts,
                                const at::Tensor& offsets, const at::Tensor& row_of,
                                int64_t capacity, const std::optional<at::Tensor>& weights) {
   TORCH_CHECK(y.dim() >= 1 && row_of.dim() == 2, "unpermute_tokens: y must be rows, row_of [tokens, topk]");
-  at::Tensor out = at::empty({row_of.size(0), y.size(-1)}, y.options());
+  at::Tensor out = empty({row_of.size(0), y.size(-1)}, y, y.scalar_type());
   unpermute_tokens_out_op(y, counts, offsets, row_of, capacity, weights, out, std::nullopt);
   return out;
 }
@@ -310,6 +316,123 @@ void unpermute_tokens_backward_op(const at::Tensor& grad, const at::Tensor& y,
     c.grad_weights = data<float>(*grad_weights);
   }
   launch_on(grad, [&](cudaStream_t stream) { launch_unpermute_backward(c, stream); });
+}
+
+// ------------------------------------------------------------------- gradients ----
+
+using Variables = torch::autograd::variable_list;
+using torch::autograd::AutogradContext;
+
+at::Tensor call_permute(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,
+                        const at::Tensor& row_of, int64_t capacity, bool zero_rest) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pplx_kernels_b200::permute_tokens", "")
+                       .typed<decltype(permute_tokens_op)>();
+  return op.call(x, counts, offsets, row_of, capacity, zero_rest);
+}
+
+at::Tensor call_unpermute(const at::Tensor& y, const at::Tensor& counts, const at::Tensor& offsets,
+                          const at::Tensor& row_of, int64_t capacity,
+                          const std::optional<at::Tensor>& weights) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pplx_kernels_b200::unpermute_tokens", "")
+                       .typed<decltype(unpermute_tokens_op)>();
+  return op.call(y, counts, offsets, row_of, capacity, weights);
+}
+
+void call_unpermute_backward(const at::Tensor& grad, const at::Tensor& y, const at::Tensor& counts,
+                             const at::Tensor& offsets, const at::Tensor& row_of, int64_t capacity,
+                             const at::Tensor& weights, const std::optional<at::Tensor>& grad_y,
+                             const std::optional<at::Tensor>& grad_weights) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pplx_kernels_b200::unpermute_tokens_backward", "")
+                       .typed<decltype(unpermute_tokens_backward_op)>();
+  op.call(grad, y, counts, offsets, row_of, capacity, weights, grad_y, grad_weights);
+}
+
+// Rows without a token are zero where a gradient is recorded: what is computed with them may enter
+// the gradients of weights, multiplied by zeros.
+class Permute : public torch::autograd::Function<Permute> {
+ public:
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& counts,
+                            const at::Tensor& offsets, const at::Tensor& row_of, int64_t capacity) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({counts, offsets, row_of});
+    ctx->saved_data["capacity"] = capacity;
+    return call_permute(x, counts, offsets, row_of, capacity, true);
+  }
+  static Variables backward(AutogradContext* ctx, const Variables& grads) {
+    const Variables rows = ctx->get_saved_variables();
+    return {call_unpermute(grads[0].contiguous(), rows[0], rows[1], rows[2],
+                           ctx->saved_data["capacity"].toInt(), std::nullopt),
+            {}, {}, {}, {}};
+  }
+};
+
+class Unpermute : public torch::autograd::Function<Unpermute> {
+ public:
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& weights,
+                            const at::Tensor& counts, const at::Tensor& offsets,
+                            const at::Tensor& row_of, int64_t capacity) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({y, weights, counts, offsets, row_of});
+    ctx->saved_data["capacity"] = capacity;
+    return call_unpermute(y, counts, offsets, row_of, capacity, weights);
+  }
+  static Variables backward(AutogradContext* ctx, const Variables& grads) {
+    const Variables saved = ctx->get_saved_variables();
+    const at::Tensor &y = saved[0], &weights = saved[1];
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "unpermute_tokens: its gradient has no derivative of its own (create_graph)");
+    at::Tensor grad_y, grad_weights;
+    if (ctx->needs_input_grad(0)) grad_y = at::empty_like(y);
+    if (ctx->needs_input_grad(1)) grad_weights = at::empty_like(weights);
+    auto given = [](const at::Tensor& t) {
+      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    };
+    call_unpermute_backward(grads[0].contiguous(), y, saved[2], saved[3], saved[4],
+                            ctx->saved_data["capacity"].toInt(), weights, given(grad_y),
+                            given(grad_weights));
+    return {grad_y, grad_weights, {}, {}, {}, {}};
+  }
+};
+
+class Sum : public torch::autograd::Function<Sum> {  // unpermute without weights
+ public:
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& counts,
+                            const at::Tensor& offsets, const at::Tensor& row_of, int64_t capacity) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({counts, offsets, row_of});
+    ctx->saved_data["capacity"] = capacity;
+    return call_unpermute(y, counts, offsets, row_of, capacity, std::nullopt);
+  }
+  static Variables backward(AutogradContext* ctx, const Variables& grads) {
+    const Variables rows = ctx->get_saved_variables();
+    return {call_permute(grads[0].contiguous(), rows[0], rows[1], rows[2],
+                         ctx->saved_data["capacity"].toInt(), true),
+            {}, {}, {}, {}};
+  }
+};
+
+at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts,
+                                   const at::Tensor& offsets, const at::Tensor& row_of,
+                                   int64_t capacity, bool zero_rest) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return Permute::apply(x, counts, offsets, row_of, capacity);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_permute(x, counts, offsets, row_of, capacity, zero_rest);
+}
+
+at::Tensor unpermute_tokens_autograd(const at::Tensor& y, const at::Tensor& counts,
+                                     const at::Tensor& offsets, const at::Tensor& row_of,
+                                     int64_t capacity, const std::optional<at::Tensor>& weights) {
+  if (at::GradMode::is_enabled()) {
+    if (weights.has_value() && (y.requires_grad() || weights->requires_grad()))
+      return Unpermute::apply(y, *weights, counts, offsets, row_of, capacity);
+    if (y.requires_grad()) return Sum::apply(y, counts, offsets, row_of, capacity);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_unpermute(y, counts, offsets, row_of, capacity, weights);
 }
 
 // -------------------------------------------------------------------- int8 ----
@@ -358,8 +481,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows_int8_op(const at::Tensor& x,
                                                          const std::optional<at::Tensor>& counts) {
   TORCH_CHECK(x.dim() == 2 || x.dim() == 3,
               "quantize_rows_int8: x must be [rows, k] or [experts, rows, k]");
-  at::Tensor out = at::empty(x.sizes(), x.options().dtype(at::kChar));
-  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  at::Tensor out = empty(x.sizes(), x, at::kChar);
+  at::Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
   quantize_rows_int8_out_op(x, counts, out, scale);
   return {out, scale};
 }
@@ -470,6 +593,7 @@ void register_expert_ops(torch::Library& m) {
         "bool zero_rest) -> Tensor");
   m.impl("permute_tokens", c10::kCUDA, &permute_tokens_op);
   m.impl("permute_tokens", c10::kMeta, &permute_tokens_op);
+  m.impl("permute_tokens", torch::dispatch(c10::DispatchKey::Autograd, &permute_tokens_autograd));
   m.def("permute_tokens_out(Tensor x, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
         "Tensor! out, bool zero_rest) -> ()");
   m.impl("permute_tokens_out", c10::kCUDA, &permute_tokens_out_op);
@@ -486,6 +610,7 @@ void register_expert_ops(torch::Library& m) {
         "Tensor? weights) -> Tensor");
   m.impl("unpermute_tokens", c10::kCUDA, &unpermute_tokens_op);
   m.impl("unpermute_tokens", c10::kMeta, &unpermute_tokens_op);
+  m.impl("unpermute_tokens", torch::dispatch(c10::DispatchKey::Autograd, &unpermute_tokens_autograd));
   m.def("unpermute_tokens_out(Tensor y, Tensor counts, Tensor offsets, Tensor row_of, int capacity, "
         "Tensor? weights, Tensor! out, Tensor? bound_m) -> ()");
   m.impl("unpermute_tokens_out", c10::kCUDA, &unpermute_tokens_out_op);

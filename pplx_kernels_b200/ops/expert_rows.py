@@ -23,7 +23,6 @@ Nothing here synchronises with the host: all of it can be captured in a CUDA gra
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ops
 
@@ -64,21 +63,6 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, capacity: int = 0,
     return ExpertRows(counts, offsets, row_of, capacity, bound_m)
 
 
-class _Permute(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, counts, offsets, row_of, capacity):
-        ctx.save_for_backward(counts, offsets, row_of)
-        ctx.capacity = capacity
-        return _ops.permute_tokens(x, counts, offsets, row_of, capacity, True)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        return (permute_tokens_backward(grad.contiguous(),
-                                        ExpertRows(*ctx.saved_tensors, ctx.capacity)),
-                None, None, None, None)
-
-
 def permute_tokens(x: torch.Tensor, rows: ExpertRows, zero_rest: bool | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """Copies every token of ``x`` [tokens, hidden] to its rows: ``out[rows.row_of[t, k]] = x[t]``.
@@ -92,7 +76,6 @@ def permute_tokens(x: torch.Tensor, rows: ExpertRows, zero_rest: bool | None = N
             raise ValueError("permute_tokens: rows without a token are zero where a gradient is recorded")
         if out is not None:
             raise _no_gradient("permute_tokens")
-        return _Permute.apply(x, rows.counts, rows.offsets, rows.row_of, rows.capacity)
     if out is None:
         return _ops.permute_tokens(x, rows.counts, rows.offsets, rows.row_of, rows.capacity,
                                    bool(zero_rest))
@@ -125,24 +108,6 @@ def permute_tokens_int8(x: torch.Tensor, rows: ExpertRows, zero_rest: bool = Fal
     return out, out_scale
 
 
-class _Unpermute(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, counts, offsets, row_of, capacity):
-        ctx.save_for_backward(y, weights, counts, offsets, row_of)
-        ctx.capacity = capacity
-        return _ops.unpermute_tokens(y, counts, offsets, row_of, capacity, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        y, weights, counts, offsets, row_of = ctx.saved_tensors
-        need_y, need_w = ctx.needs_input_grad[:2]
-        grad_y, grad_weights = unpermute_tokens_backward(
-            grad if grad.is_contiguous() else grad.contiguous(), y,
-            ExpertRows(counts, offsets, row_of, ctx.capacity), weights, need_y, need_w)
-        return grad_y, grad_weights, None, None, None, None
-
-
 def unpermute_tokens(y: torch.Tensor, rows: ExpertRows, weights: torch.Tensor | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Sums each token's rows: ``out[t] = sum over k of weights[t, k] * y[rows.row_of[t, k]]``.
@@ -152,16 +117,12 @@ def unpermute_tokens(y: torch.Tensor, rows: ExpertRows, weights: torch.Tensor | 
     without rows is zero.  Where the routing was sorted with ``bound_m``, an ``out`` that is given
     keeps its rows at or beyond it; they are zero in one that is allocated here.
 
-    Differentiable in ``y`` and ``weights``; the gradient of rows without a token is zero.
+    Differentiable, once, in ``y`` and ``weights``; the gradient of rows without a token is zero.
     """
-    if (y.requires_grad or (weights is not None and weights.requires_grad)) and torch.is_grad_enabled():
-        if out is not None:
-            raise _no_gradient("unpermute_tokens")
-        if weights is None:
-            weights = torch.ones(rows.row_of.shape, dtype=torch.float32, device=y.device)
-        return _Unpermute.apply(y, weights, rows.counts, rows.offsets, rows.row_of, rows.capacity)
     if out is None:
         return _ops.unpermute_tokens(y, rows.counts, rows.offsets, rows.row_of, rows.capacity, weights)
+    if (y.requires_grad or (weights is not None and weights.requires_grad)) and torch.is_grad_enabled():
+        raise _no_gradient("unpermute_tokens")
     _ops.unpermute_tokens_out(y, rows.counts, rows.offsets, rows.row_of, rows.capacity, weights, out,
                               rows.bound_m)
     return out
