@@ -60,6 +60,7 @@ constexpr uint32_t kWBytes = kBlockM * kRowBytes;
 constexpr uint32_t kWaitLimitNs = 2000000000u;  // 2 s per wait
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 131071;
+constexpr int kTable = 32;        // tiles of a worker that are looked up in advance
 constexpr int kDrain = 22;        // cycles per token row to read out an accumulator that is the only one
 
 struct Int8GemmArgs {
@@ -89,6 +90,7 @@ struct Control {
   uint32_t max_rows;
   uint32_t max_width;
   unsigned long long best_limit;
+  Tile tiles[kTable];
   alignas(128) uint8_t seg[8][32 * 64];  // of each epilogue warp: 32 tokens' columns
   alignas(16) float sx[2][kMaxTokens];  // scales of a tile's tokens, of two tiles in turn
 };
@@ -220,13 +222,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (warp == 0) warp_exclusive_scan_smem(tile_start, g.num_experts, lane, true);
+  __syncthreads();
+  // The search for a tile takes one thread some 500 cycles: those of this worker's first tiles are
+  // made side by side.
+  const uint32_t total_tiles = tile_start[g.num_experts];
+  if (tid < kTable && worker + tid * workers < total_tiles)
+    ctl->tiles[tid] = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, worker + tid * workers);
+  auto tile = [&](uint32_t local) {
+    return local < kTable ? ctl->tiles[local]
+                          : locate<kUnit>(tile_start, rows_of, g.num_experts, limit,
+                                          worker + local * workers);
+  };
   tc::tc_fence_before_sync();
   __syncthreads();
   // The peer must see initialised barriers before anything arrives on them remotely.
   if constexpr (kPair) tc::cluster_sync();
   tc::tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
-  const uint32_t total_tiles = tile_start[g.num_experts];
   // As many stages as the launch's widest token tile leaves room for.
   const uint32_t stage_bytes = kWBytes + ctl->max_width / kCtas * kRowBytes;
   const uint32_t stages = min(g.ring_bytes / stage_bytes, static_cast<uint32_t>(kMaxStages));
@@ -238,9 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t stage = 0, phase = 0;
       uint32_t pending = 0;        // stages that have been filled at least once
       uint32_t pending_phase = 0;  // parity of the phase each stage was last filled in
+      uint32_t local = 0;
       bool ok = *abort_flag == 0u;
-      for (uint32_t t = worker; t < total_tiles && ok; t += workers) {
-        const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
+      for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
+        const Tile c = tile(local);
         // This CTA's share of the tokens of each MMA.
         const int n0 = kPair ? first_mma(c.width) : c.width;
         const int own0 = n0 / kCtas, own1 = (c.width - n0) / kCtas;
@@ -304,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = *abort_flag == 0u;
       for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
-        const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
+        const Tile c = tile(local);
         const int n0 = kPair ? first_mma(c.width) : c.width, n1 = c.width - n0;
         const uint32_t idesc = tc::make_instr_desc_i8(kBlockM * kCtas, n0);
         const uint32_t idesc1 = tc::make_instr_desc_i8(kBlockM * kCtas, n1);
@@ -359,26 +372,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
     uint32_t local = 0;
     bool ok = *abort_flag == 0u;
+    // A tile's scales are on their way while the tile before is finished.  sw, plain: weight rows
+    // lane / 4 + 0, 8, 16, 24 of the warp; SwiGLU: gate and up of two columns.
+    float next_sx[2], next_sw[4];
+    auto fetch_scales = [&](const Tile& c) {
+      const int live = min(c.width, c.rows - c.first);
+      const float* sx = g.sx + c.expert * g.sx_stride_e + row0_of[c.expert] + c.first;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) next_sx[i] = n_tid + 256 * i < live ? sx[n_tid + 256 * i] : 0.0f;
+      const float* sw = g.sw + c.expert * g.sw_stride_e;
+      const int col = (c.w_blk * kCtas + static_cast<int>(cta_rank)) * kCols + kWarpCols * ew + (lane >> 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = SWIGLU ? col + (i >> 1) * 8 : col + i * 8;
+        next_sw[i] = at < g.n_out ? sw[SWIGLU && (i & 1) ? g.n_out + at : at] : 0.0f;
+      }
+    };
+    if (worker < total_tiles) fetch_scales(tile(0));
     for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
-      const Tile c = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, t);
+      const Tile c = tile(local);
       const int live = min(c.width, c.rows - c.first);  // tokens of the tile that exist
       const int col0 = (c.w_blk * kCtas + static_cast<int>(cta_rank)) * kCols;
       const int64_t row0 = static_cast<int64_t>(row0_of[c.expert]) + c.first;
-      // The tile's scales, while its MMAs run.  (The table of the tile before is still read: the
-      // barrier below is what ends that.)
+      // (The table of the tile before is still read: the barrier below is what ends that.)
       float* sx = ctl->sx[local & 1u];
-      for (int n = n_tid; n < c.width; n += 256)
-        sx[n] = n < live ? g.sx[c.expert * g.sx_stride_e + row0 + n] : 0.0f;
-      float sw[4];  // plain: weight rows lane / 4 + 0, 8, 16, 24; SwiGLU: gate, up of two columns
-      {
-        const float* s = g.sw + c.expert * g.sw_stride_e;
-        const int col = col0 + kWarpCols * ew + (lane >> 2);
+      sx[n_tid] = next_sx[0];
+      sx[n_tid + 256] = next_sx[1];
+      float sw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = SWIGLU ? col + (i >> 1) * 8 : col + i * 8;
-          sw[i] = at < g.n_out ? s[SWIGLU && (i & 1) ? g.n_out + at : at] : 0.0f;
-        }
-      }
+      for (int i = 0; i < 4; ++i) sw[i] = next_sw[i];
       // Where this thread stores: token lane / kPieces of every 32 / kPieces, 16 bytes.
       const int store_token = lane / kPieces, store_piece = lane % kPieces;
       const int store_col = col0 + kWarpCols * ew + store_piece * 8;
@@ -404,6 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       tc::tc_fence_after_sync();
+      if (t + workers < total_tiles) fetch_scales(tile(local + 1));
       const int groups = (c.width + 31) >> 5;
       const uint32_t t_acc = t_lane + buf * kMmaTokens;
       // The accumulator is handed back when the warp has its last columns in registers.

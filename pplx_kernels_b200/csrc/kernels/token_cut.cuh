@@ -31,8 +31,13 @@ template <int kUnit>
 struct Cut {
   int units, tiles;
   __device__ __forceinline__ Cut(int rows, int limit)
-      : units((rows + kUnit - 1) / kUnit), tiles((units * kUnit + limit - 1) / limit) {}
-  __device__ __forceinline__ int widest() const { return (units + tiles - 1) / tiles * kUnit; }
+      : units((rows + kUnit - 1) / kUnit),
+        // (Divisions by numbers that only the device knows take hundreds of cycles; most experts have
+        // one tile.)
+        tiles(units * kUnit <= limit ? min(units, 1) : (units * kUnit + limit - 1) / limit) {}
+  __device__ __forceinline__ int widest() const {
+    return (tiles == 1 ? units : (units + tiles - 1) / tiles) * kUnit;
+  }
 };
 
 template <int kUnit>
@@ -43,6 +48,12 @@ __device__ __forceinline__ Tile locate(const uint32_t* tile_start, const uint32_
   c.rows = static_cast<int>(rows_of[c.expert]);
   const Cut<kUnit> cut(c.rows, limit);
   const uint32_t rem = t - tile_start[c.expert];
+  if (cut.tiles == 1) {
+    c.w_blk = static_cast<int>(rem);
+    c.first = 0;
+    c.width = cut.units * kUnit;
+    return c;
+  }
   c.w_blk = static_cast<int>(rem / cut.tiles);
   const int i = static_cast<int>(rem) - c.w_blk * cut.tiles;
   const int each = cut.units / cut.tiles, wider = cut.units - each * cut.tiles;
