@@ -12,19 +12,19 @@
 // the work follows the rows there are; a stage of 128 bytes of K holds 128 integers, twice what a
 // stage of the bf16 kernel holds.  A CTA owns a tile of 128 weight rows times a token tile of 16
 // to 256 rows of one expert; or a CTA pair (cta_group::2) 256 weight rows, 128 in each CTA, times 32
-// to 512, of which each CTA loads half (above 256 as two MMAs that share the weights).  No TMA
+// to 512, of which each CTA loads half (wide tiles as two halves that share the weights).  No TMA
 // multicast is involved.
 //
 // What bounds it, at 6.5 TB/s of HBM and 3.36 POPS (twice the bf16 rate): the weights' bytes up to
-// some 128 rows per expert (32 experts of 2048 x 7168, up projection, 64 rows each: 144 us, floor 147
+// some 128 rows per expert (32 experts of 2048 x 7168, up projection, 64 rows each: 145 us, floor 147
 // with the rows), L2 around 256 rows (175 us, floor 158), the tensor cores and the power limit above
 // (1024 rows: 600 us = 3.2 POPS; 8 experts of 4096 x 14336, down, 1024 rows: 296 us).  An epilogue that
 // divided by the IEEE quotient and met two barriers per 16 tokens bound the tiles with short K: 128
-// experts of 768 x 2048, up, 256 rows 191 us, now 92; down 77 -> 68.
+// experts of 768 x 2048, up, 256 rows 191 us, now 91; down 77 -> 65.
 //
 // Roles (persistent over tiles): warp 0 TMA producer, warp 1 MMA issuer (leader CTA only), warp 2
 // tensor-memory allocation, warps 4-11 epilogue.  Two accumulators of 256 columns let the epilogue
-// of a tile run under the MMAs of the next; wider tiles have one of 512.  Every mbarrier wait is bounded: when one runs out the CTA raises a
+// of a tile run under the MMAs of the next; for wider tiles see below.  Every mbarrier wait is bounded: when one runs out the CTA raises a
 // shared abort flag, all roles leave their loops, in-flight TMA loads are drained, tensor memory is
 // freed and the kernel returns with *status = 1.
 #include <algorithm>
@@ -54,14 +54,15 @@ constexpr int kBlockK = 128;      // integers = bytes: one 128-byte swizzle row
 constexpr int kUmmaK = 32;
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 384;
-constexpr int kTmemCols = 512;    // an accumulator of kMaxTokens columns, or two of half of them
+constexpr int kTmemCols = 512;
 constexpr uint32_t kRowBytes = kBlockK;
 constexpr uint32_t kWBytes = kBlockM * kRowBytes;
 constexpr uint32_t kWaitLimitNs = 2000000000u;  // 2 s per wait
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 131071;
+constexpr int kMaxSlots = 3;       // accumulators in tensor memory
+constexpr int kThirdCols = 160;    // columns of each where there are three
 constexpr int kTable = 32;        // tiles of a worker that are looked up in advance
-constexpr int kDrain = 22;        // cycles per token row to read out an accumulator that is the only one
 
 struct Int8GemmArgs {
   const int32_t* counts;   // [num_experts] valid rows per expert; null: rows_per_expert
@@ -83,8 +84,8 @@ struct Int8GemmArgs {
 struct Control {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t tmem_full[2];
-  uint64_t tmem_empty[2];
+  uint64_t tmem_full[kMaxSlots];
+  uint64_t tmem_empty[kMaxSlots];
   uint32_t tmem_base;
   uint32_t abort_flag;
   uint32_t max_rows;
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&ctl->full[s], 1);
       tc::mbar_init(&ctl->empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kMaxSlots; ++b) {
       tc::mbar_init(&ctl->tmem_full[b], 1);
       tc::mbar_init(&ctl->tmem_empty[b], 8 * kCtas);  // epilogue warps of the tile
     }
@@ -187,12 +188,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   // The most token rows a tile may have.  One tile per expert up to 256 rows: there an expert is
   // bound by its weights, which more tiles would only read again.  Above, the limit that
-  // minimises (waves of tiles) x (time of a tile).  A tile of w rows was measured to take 330 + 5/3 w
-  // cycles per K block of 128 bytes up to 256 rows and 220 + 11/5 w above (fewer stages): more than
-  // the 2 w cycles of its MMAs, because L2 delivers some 42 bytes per cycle and SM, of 16 KB of
-  // weights and 64 w bytes of tokens.  More than 256 rows leave no second accumulator, so their
-  // epilogue is not hidden.  Every CTA computes the same.  (32 experts of 2048 x 7168, up projection,
-  // 320 rows each: one tile of 320 213 us, two of 160 246 us; 384: 244, 274 us; 512: 312, 313 us.)
+  // minimises (waves of tiles) x (time of a tile).  Measured, in cycles per K block of 128 bytes of a
+  // tile of w rows: 330 + 5/3 w up to 256 rows, 220 + 11/5 w up to 384 and 18/5 w - 340 above (there
+  // are fewer stages); more than the 2 w cycles of its MMAs, because L2 delivers some 42 bytes per
+  // cycle and SM, of 16 KB of weights and 64 w bytes of tokens.  And the epilogue of more than 256 rows
+  // is not hidden as a whole: 6 cycles per row with three accumulators, 10 with two.  Every CTA computes
+  // the same.  (us for one tile of all rows and two of half of them: 32 experts of 2048 x 7168, up, 320
+  // rows each 206, 255; 384: 241, 283; 512: 308, 310; down 320 rows 130, 141; 512: 199, 171.)
   int limit = kPair ? kMaxTokens : kMmaTokens;
   if (ctl->max_rows > kMmaTokens) {
     for (int cand = limit - kUnit * warp; 4 * cand >= limit; cand -= kUnit * (kThreads / 32)) {
@@ -207,8 +209,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         const uint64_t waves = ceil_div<uint64_t>(static_cast<uint64_t>(tiles) * w_blocks, workers);
         const uint32_t w = width / tiles;
-        const uint64_t each = max(330u + 5u * w / 3u, 220u + 11u * w / 5u);
-        const uint64_t cost = waves * (num_kb * each + (cand > kMmaTokens ? kDrain * w : 0u));
+        const uint64_t each = max(max(330u + 5u * w / 3u, 220u + 11u * w / 5u), 18u * max(w, 100u) / 5u - 340u);
+        const uint32_t drain = cand <= kMmaTokens ? 0u : cand <= 2 * kThirdCols ? 6u : 10u;
+        const uint64_t cost = waves * (num_kb * each + drain * w);
         atomicMin(&ctl->best_limit, (cost << 16) | static_cast<uint64_t>(kMaxTokens - cand));
       }
     }
@@ -242,7 +245,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   // As many stages as the launch's widest token tile leaves room for.
   const uint32_t stage_bytes = kWBytes + ctl->max_width / kCtas * kRowBytes;
   const uint32_t stages = min(g.ring_bytes / stage_bytes, static_cast<uint32_t>(kMaxStages));
-  const bool two = !kPair || ctl->max_width <= kMmaTokens;  // two accumulators
+  // Accumulators are slots of tensor memory that the MMAs take in turn: two of 256 columns, or three
+  // of 160 where a tile is wider than 256 rows, but none than 320.  A tile that is wider than a slot is
+  // two halves, each with its MMAs and a slot of its own, so that the MMAs of a tile can begin while
+  // the second half (with three: both) of the tile before is read out.
+  const bool thirds = kPair && ctl->max_width > kMmaTokens && ctl->max_width <= 2 * kThirdCols;
+  const int slot_cols = thirds ? kThirdCols : kMmaTokens;
+  const uint32_t slots = thirds ? 3u : 2u;
+  auto first_half = [&](int width) {
+    return !kPair || width <= slot_cols ? width : ((width >> 1) + 31) & ~31;
+  };
 
   // ---- roles ----------------------------------------------------------------
   if (warp == 0) {
@@ -255,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
         const Tile c = tile(local);
         // This CTA's share of the tokens of each MMA.
-        const int n0 = kPair ? first_mma(c.width) : c.width;
+        const int n0 = first_half(c.width);
         const int own0 = n0 / kCtas, own1 = (c.width - n0) / kCtas;
         const int tile_row = static_cast<int>(row0_of[c.expert]) + c.first;
         const int row0 = tile_row + static_cast<int>(cta_rank) * own0;
@@ -315,53 +327,83 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (leader && tc::elect_one()) {
       uint32_t stage = 0, phase = 0, local = 0;
+      uint32_t slot = 0, lap = 0;  // the next accumulator, and the parity of its use
+      auto next_slot = [&] {
+        if (++slot == slots) slot = 0, lap ^= 1u;
+      };
+      auto next_stage = [&](uint32_t& at, uint32_t& parity) {
+        if (++at == stages) at = 0, parity ^= 1u;
+      };
       bool ok = *abort_flag == 0u;
       for (uint32_t t = worker; t < total_tiles && ok; t += workers, ++local) {
         const Tile c = tile(local);
-        const int n0 = kPair ? first_mma(c.width) : c.width, n1 = c.width - n0;
+        const int n0 = first_half(c.width), n1 = c.width - n0;
         const uint32_t idesc = tc::make_instr_desc_i8(kBlockM * kCtas, n0);
         const uint32_t idesc1 = tc::make_instr_desc_i8(kBlockM * kCtas, n1);
-        const uint32_t buf = two ? local & 1u : 0u;
-        const uint32_t use = two ? local >> 1 : local;  // how often this accumulator was used before
-        ok = tc::mbar_wait(&ctl->tmem_empty[buf], (use & 1u) ^ 1u, abort_flag, kWaitLimitNs);
+        const uint32_t slot0 = slot, lap0 = lap;
+        next_slot();
+        ok = tc::mbar_wait(&ctl->tmem_empty[slot0], lap0 ^ 1u, abort_flag, kWaitLimitNs);
         if (!ok) break;
         tc::tc_fence_after_sync();
-        const uint32_t tmem_d = tmem_base + buf * kMmaTokens;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          ok = tc::mbar_wait(&ctl->full[stage], phase, abort_flag, kWaitLimitNs);
-          if (!ok) break;
-          tc::tc_fence_after_sync();
-          const uint8_t* w_src = ring + stage * stage_bytes;
+        // One half's MMAs of a K block.
+        auto multiply = [&](uint32_t stage_at, uint32_t x_off, uint32_t tmem_d, uint32_t desc, int kb) {
+          const uint8_t* w_src = ring + stage_at * stage_bytes;
           const uint64_t w_desc = tc::make_smem_desc_sw128(w_src);
-          const uint64_t x_desc = tc::make_smem_desc_sw128(w_src + kWBytes);
+          const uint64_t x_desc = tc::make_smem_desc_sw128(w_src + kWBytes + x_off);
 #pragma unroll
           for (int k = 0; k < kBlockK / kUmmaK; ++k) {
             const uint64_t wd = tc::advance_smem_desc(w_desc, k * kUmmaK);
             const uint64_t xd = tc::advance_smem_desc(x_desc, k * kUmmaK);
-            if constexpr (kPair) tc::mma_i8_ss_2cta(tmem_d, wd, xd, idesc, (kb | k) != 0);
-            else tc::mma_i8_ss(tmem_d, wd, xd, idesc, (kb | k) != 0);
+            if constexpr (kPair) tc::mma_i8_ss_2cta(tmem_d, wd, xd, desc, (kb | k) != 0);
+            else tc::mma_i8_ss(tmem_d, wd, xd, desc, (kb | k) != 0);
           }
-          if constexpr (kPair) {
-            if (n1 > 0) {
-              const uint64_t x1_desc = tc::advance_smem_desc(x_desc, n0 / kCtas * kRowBytes);
-#pragma unroll
-              for (int k = 0; k < kBlockK / kUmmaK; ++k)
-                tc::mma_i8_ss_2cta(tmem_d + n0, tc::advance_smem_desc(w_desc, k * kUmmaK),
-                                   tc::advance_smem_desc(x1_desc, k * kUmmaK), idesc1, (kb | k) != 0);
-            }
+        };
+        auto commit = [&](uint64_t* bar) {  // in both CTAs of a pair
+          if constexpr (kPair) tc::mma_commit_2cta(bar, 0x3);
+          else tc::mma_commit(bar);
+        };
+        const uint32_t tmem0 = tmem_base + slot0 * slot_cols;
+        if (!kPair || n1 == 0) {
+          for (int kb = 0; kb < num_kb; ++kb) {
+            ok = tc::mbar_wait(&ctl->full[stage], phase, abort_flag, kWaitLimitNs);
+            if (!ok) break;
+            tc::tc_fence_after_sync();
+            multiply(stage, 0, tmem0, idesc, kb);
+            commit(&ctl->empty[stage]);  // reusable once these MMAs have read it
+            next_stage(stage, phase);
           }
-          // Stage reusable (in both CTAs of a pair) once these MMAs have read it.
-          if constexpr (kPair) tc::mma_commit_2cta(&ctl->empty[stage], 0x3);
-          else tc::mma_commit(&ctl->empty[stage]);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
+          if (ok) commit(&ctl->tmem_full[slot0]);
+          continue;
+        }
+        // Two halves: the first goes ahead, up to all stages, until the second's slot is free.
+        const uint32_t slot1 = slot, lap1 = lap;
+        next_slot();
+        const uint32_t tmem1 = tmem_base + slot1 * slot_cols;
+        uint32_t stage1 = stage, phase1 = phase;
+        bool free1 = false;
+        for (int kb0 = 0, kb1 = 0; kb1 < num_kb;) {
+          if (!free1 && tc::mbar_try_wait(&ctl->tmem_empty[slot1], lap1 ^ 1u)) {
+            free1 = true;
+            tc::tc_fence_after_sync();
+          }
+          if (free1 && kb1 < kb0) {
+            multiply(stage1, n0 / kCtas * kRowBytes, tmem1, idesc1, kb1);
+            commit(&ctl->empty[stage1]);
+            next_stage(stage1, phase1);
+            ++kb1;
+          } else if (kb0 < num_kb && kb0 - kb1 < static_cast<int>(stages)) {
+            ok = tc::mbar_wait(&ctl->full[stage], phase, abort_flag, kWaitLimitNs);
+            if (!ok) break;
+            tc::tc_fence_after_sync();
+            multiply(stage, 0, tmem0, idesc, kb0);
+            next_stage(stage, phase);
+            if (++kb0 == num_kb) commit(&ctl->tmem_full[slot0]);
+          } else {
+            ok = tc::mbar_wait(&ctl->tmem_empty[slot1], lap1 ^ 1u, abort_flag, kWaitLimitNs);
+            if (!ok) break;
           }
         }
-        if (ok) {
-          if constexpr (kPair) tc::mma_commit_2cta(&ctl->tmem_full[buf], 0x3);
-          else tc::mma_commit(&ctl->tmem_full[buf]);
-        }
+        if (ok) commit(&ctl->tmem_full[slot1]);
       }
     }
     __syncwarp();
@@ -371,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_tid = tid - 128;     // over the epilogue warps
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
     uint32_t local = 0;
+    uint32_t slot = 0, lap = 0;  // the next accumulator, and the parity of its use
     bool ok = *abort_flag == 0u;
     // A tile's scales are on their way while the tile before is finished.  sw, plain: weight rows
     // lane / 4 + 0, 8, 16, 24 of the warp; SwiGLU: gate and up of two columns.
@@ -394,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int live = min(c.width, c.rows - c.first);  // tokens of the tile that exist
       const int col0 = (c.w_blk * kCtas + static_cast<int>(cta_rank)) * kCols;
       const int64_t row0 = static_cast<int64_t>(row0_of[c.expert]) + c.first;
-      // (The table of the tile before is still read: the barrier below is what ends that.)
+      // (The table of the tile before is still read: the barriers below are what ends that.)
       float* sx = ctl->sx[local & 1u];
       sx[n_tid] = next_sx[0];
       sx[n_tid + 256] = next_sx[1];
@@ -406,38 +449,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int store_col = col0 + kWarpCols * ew + store_piece * 8;
       uint16_t* out = g.out + c.expert * g.out_stride_e + row0 * g.out_stride_row + store_col;
       const int stored = store_col + 8 <= g.n_out ? live : 0;
-      const uint32_t buf = two ? local & 1u : 0u;
-      ok = tc::mbar_wait(&ctl->tmem_full[buf], (two ? local >> 1 : local) & 1u, abort_flag, kWaitLimitNs);
-      // All eight warps leave together or not at all: the barriers below must never be
-      // entered by only some of them.
-      {
-        uint32_t all_ok;
-        asm volatile(
-            "{\n\t"
-            ".reg .pred p, q;\n\t"
-            "setp.ne.u32 q, %1, 0;\n\t"
-            "bar.red.and.pred p, 1, %2, q;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t"
-            "}\n"
-            : "=r"(all_ok)
-            : "r"(ok ? 1u : 0u), "n"(256)
-            : "memory");
-        ok = all_ok != 0u;
-      }
-      if (!ok) break;
-      tc::tc_fence_after_sync();
-      if (t + workers < total_tiles) fetch_scales(tile(local + 1));
-      const int groups = (c.width + 31) >> 5;
-      const uint32_t t_acc = t_lane + buf * kMmaTokens;
-      // The accumulator is handed back when the warp has its last columns in registers.
-      auto hand_back = [&] {
-        tc::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (kPair) tc::mbar_arrive_on_leader_relaxed(&ctl->tmem_empty[buf]);
-          else tc::mbar_arrive(&ctl->tmem_empty[buf]);
-        }
-      };
       // 32 tokens at a time, the next ones on their way while these are finished.  A thread's values
       // lie across token rows; they pass through shared memory of the warp's own, so that rows leave
       // in 16-byte pieces.  (The pieces of a row of shared memory are in an order that keeps both
@@ -446,14 +457,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto at = [&](int token, int piece) {
         return seg + token * (kPieces * 16) + ((piece ^ (token / (8 / kPieces) % kPieces)) * 16);
       };
-      auto finish = [&](int grp, const uint32_t (&lo)[16], const uint32_t (&hi)[16]) {
+      auto finish = [&](int n, const uint32_t (&lo)[16], const uint32_t (&hi)[16]) {
         __syncwarp();  // (the tokens before have been read)
 #pragma unroll
         for (int b = 0; b < 4; b += SWIGLU ? 2 : 1) {
-          const float2 s = *reinterpret_cast<const float2*>(&sx[grp * 32 + 8 * b + 2 * (lane & 3)]);
+          const float2 s = *reinterpret_cast<const float2*>(&sx[n + 8 * b + 2 * (lane & 3)]);
           if constexpr (SWIGLU) {
             // Lanes 0-7 of every 16 are gate rows, 8-15 the up rows of the same columns.
-            const float2 s1 = *reinterpret_cast<const float2*>(&sx[grp * 32 + 8 * b + 8 + 2 * (lane & 3)]);
+            const float2 s1 = *reinterpret_cast<const float2*>(&sx[n + 8 * b + 8 + 2 * (lane & 3)]);
             auto pair = [&](const uint32_t* v, float2 t, float gate, float up) {
               return pack(swiglu(scaled(v[0], t.x, gate), scaled(v[2], t.x, up)),
                           swiglu(scaled(v[1], t.y, gate), scaled(v[3], t.y, up)), g.fp16);
@@ -475,31 +486,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
 #pragma unroll
         for (int t0 = 0; t0 < 32; t0 += 32 / kPieces) {
-          const int n = grp * 32 + t0 + store_token;
+          const int token = n + t0 + store_token;
           const int4 v = *reinterpret_cast<const int4*>(at(t0 + store_token, store_piece));
-          if (n < stored) *reinterpret_cast<int4*>(out + n * g.out_stride_row) = v;
+          if (token < stored) *reinterpret_cast<int4*>(out + token * g.out_stride_row) = v;
         }
       };
-      uint32_t lo[2][16], hi[2][16];
-      int grp = wg;
-      auto load = [&](int which, int from) {
-        tc::tmem_ld_16x256b_x4(t_acc + from * 32, lo[which]);
-        tc::tmem_ld_16x256b_x4(t_acc + (16u << 16) + from * 32, hi[which]);
-      };
-      if (grp < groups) load(0, grp);
-      else hand_back();
-      auto step = [&](int now) {
-        tc::tmem_ld_wait(lo[now]);
-        tc::tmem_ld_wait(hi[now]);
-        if (grp + 2 < groups) load(now ^ 1, grp + 2);
+      const int n0 = first_half(c.width);
+      for (int from = 0; from < c.width && ok; from += n0) {
+        uint64_t *full = &ctl->tmem_full[slot], *empty = &ctl->tmem_empty[slot];
+        const uint32_t t_acc = t_lane + slot * slot_cols;
+        ok = tc::mbar_wait(full, lap, abort_flag, kWaitLimitNs);
+        if (++slot == slots) slot = 0, lap ^= 1u;
+        // All eight warps leave together or not at all: this barrier must never be entered by only
+        // some of them.
+        {
+          uint32_t all_ok;
+          asm volatile(
+              "{\n\t"
+              ".reg .pred p, q;\n\t"
+              "setp.ne.u32 q, %1, 0;\n\t"
+              "bar.red.and.pred p, 1, %2, q;\n\t"
+              "selp.u32 %0, 1, 0, p;\n\t"
+              "}\n"
+              : "=r"(all_ok)
+              : "r"(ok ? 1u : 0u), "n"(256)
+              : "memory");
+          ok = all_ok != 0u;
+        }
+        if (!ok) break;
+        tc::tc_fence_after_sync();
+        if (from == 0 && t + workers < total_tiles) fetch_scales(tile(local + 1));
+        // The accumulator is handed back when the warp has its last columns in registers.
+        auto hand_back = [&] {
+          tc::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kPair) tc::mbar_arrive_on_leader_relaxed(empty);
+            else tc::mbar_arrive(empty);
+          }
+        };
+        const int groups = (min(n0, c.width - from) + 31) >> 5;
+        uint32_t lo[2][16], hi[2][16];
+        int grp = wg;
+        auto load = [&](int which, int at_grp) {
+          tc::tmem_ld_16x256b_x4(t_acc + at_grp * 32, lo[which]);
+          tc::tmem_ld_16x256b_x4(t_acc + (16u << 16) + at_grp * 32, hi[which]);
+        };
+        if (grp < groups) load(0, grp);
         else hand_back();
-        finish(grp, lo[now], hi[now]);
-        grp += 2;
-      };
+        auto step = [&](int now) {
+          tc::tmem_ld_wait(lo[now]);
+          tc::tmem_ld_wait(hi[now]);
+          if (grp + 2 < groups) load(now ^ 1, grp + 2);
+          else hand_back();
+          finish(from + grp * 32, lo[now], hi[now]);
+          grp += 2;
+        };
 #pragma unroll 1
-      while (grp < groups) {
-        step(0);
-        if (grp < groups) step(1);
+        while (grp < groups) {
+          step(0);
+          if (grp < groups) step(1);
+        }
       }
     }
   }
