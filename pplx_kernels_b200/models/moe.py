@@ -264,3 +264,137 @@ def moe_reference_fp8(x: torch.Tensor, indices: torch.Tensor, weights: torch.Ten
             o = (h @ w2[e].t()).to(torch.bfloat16).to(torch.float32)
             out[sel] += o * weights[sel, k : k + 1].to(torch.float32)
     return out
+
+
+class MoELayerInt8:
+    """The same expert FFN with 8-bit integer weights and activations: one scale per output channel
+    of a weight, one per row of the activations (``quantize_rows_int8``), exact integer sums.
+
+    On one GPU no all-to-all is involved: the tokens are sorted by expert, quantised while they are
+    copied to their experts' rows, and the weighted sum of their results brings them back
+    (``sort_by_expert``, ``permute_tokens_int8``, ``unpermute_tokens``).  With several ranks the tokens
+    are quantised, dispatched as 8-bit payload with one scale each, and combined like those of the
+    other layers.  The intermediate is rounded to bf16 by the up projection before it is quantised:
+    its row's largest value is known only when the whole row is.
+    """
+
+    def __init__(self, cfg: MoEModelConfig, max_num_tokens: int, rank: int = 0,
+                 world_size: int = 1, dp_size: int = 1, device: torch.device | None = None,
+                 seed: int = 0, group_name: str = "default", init_std: float = 0.02,
+                 ata: AllToAll | None = None) -> None:
+        from ..ops.quant import quantize_rows_int8
+
+        assert cfg.num_experts % world_size == 0
+        self.cfg = cfg
+        self.rank, self.world_size, self.dp_size = rank, world_size, dp_size
+        self.max_num_tokens = max_num_tokens
+        self.device = device or torch.device("cuda", torch.cuda.current_device())
+        self.nle = cfg.num_experts // world_size
+        H, I = cfg.hidden_dim, cfg.intermediate_dim
+        dev = self.device
+        self.ata = ata
+        if ata is None and world_size > 1:
+            self.ata = AllToAll.intranode(
+                max_num_tokens, cfg.num_experts, cfg.experts_per_token, rank, world_size, dp_size,
+                H, H, 4, group_name=group_name)
+        w13, w2 = _random_expert_weights(cfg, rank * self.nle, self.nle, seed, init_std, dev)
+        self.w13_q, self.w13_s = quantize_rows_int8(w13)  # [nle, 2I, H], [nle, 2I]
+        self.w2_q, self.w2_s = quantize_rows_int8(w2)     # [nle, H, I], [nle, H]
+        del w13, w2
+        # One expert's rows after the other's, or the planes that the all-to-all delivers.
+        if self.ata is None:
+            shape: tuple[int, ...] = (max_num_tokens * cfg.experts_per_token,)
+        else:
+            shape = (self.nle, max_num_tokens * (world_size // dp_size))
+            self.x_q = torch.zeros(max_num_tokens, H, dtype=torch.int8, device=dev)
+            self.x_scale = torch.zeros(max_num_tokens, device=dev)
+        self.counts = torch.zeros(self.nle, dtype=torch.int32, device=dev)
+        self.expert_x = torch.zeros(*shape, H, dtype=torch.int8, device=dev)
+        self.expert_scale = torch.zeros(shape, device=dev)
+        self.h = torch.zeros(*shape, I, dtype=torch.bfloat16, device=dev)
+        self.h_q = torch.zeros(*shape, I, dtype=torch.int8, device=dev)
+        self.h_scale = torch.zeros(shape, device=dev)
+        self.expert_y = torch.zeros(*shape, H, dtype=torch.bfloat16, device=dev)
+        self.gemm_status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def forward(self, x: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor,
+                out: torch.Tensor | None = None,
+                bound_m: torch.Tensor | None = None) -> torch.Tensor:
+        """x: [m, hidden] bf16; indices: [m, top-k] uint32; weights: [m, top-k] fp32."""
+        from ..ops.expert_rows import permute_tokens_int8, sort_by_expert, unpermute_tokens
+        from ..ops.grouped_gemm import grouped_gemm_int8
+        from ..ops.quant import quantize_rows_int8
+
+        m = x.size(0)
+        if m > self.max_num_tokens:
+            raise ValueError(f"MoELayerInt8: {m} tokens, room for {self.max_num_tokens}")
+        if out is None:
+            out = torch.empty(self.max_num_tokens, self.cfg.hidden_dim, dtype=torch.bfloat16,
+                              device=self.device)
+        # (As in MoELayer.forward: a hint.)
+        expect = m * self.cfg.experts_per_token * (self.world_size // self.dp_size) // self.world_size
+        if self.ata is not None:
+            q, scale = quantize_rows_int8(x, out=self.x_q[:m], out_scale=self.x_scale[:m])
+            self.ata.dispatch(self.counts, self.expert_x, self.expert_scale.unsqueeze(-1), q,
+                              scale.unsqueeze(-1), indices, bound_m)
+            grouped_gemm_int8(self.expert_x, self.expert_scale, self.w13_q, self.w13_s, self.counts,
+                              swiglu=True, out=self.h, status=self.gemm_status, expected_rows=expect)
+            quantize_rows_int8(self.h, self.counts, out=self.h_q, out_scale=self.h_scale)
+            grouped_gemm_int8(self.h_q, self.h_scale, self.w2_q, self.w2_s, self.counts,
+                              out=self.expert_y, status=self.gemm_status, expected_rows=expect)
+            self.ata.combine(out, indices, weights, self.expert_y, bound_m)
+            return out
+        rows = sort_by_expert(indices, self.nle, bound_m=bound_m)
+        n = m * self.cfg.experts_per_token
+        permute_tokens_int8(x, rows, out=self.expert_x[:n], out_scale=self.expert_scale[:n])
+        grouped_gemm_int8(self.expert_x[:n], self.expert_scale[:n], self.w13_q, self.w13_s,
+                          rows.counts, rows.offsets, swiglu=True, out=self.h[:n],
+                          status=self.gemm_status, expected_rows=expect)
+        quantize_rows_int8(self.h[:n], out=self.h_q[:n], out_scale=self.h_scale[:n])
+        grouped_gemm_int8(self.h_q[:n], self.h_scale[:n], self.w2_q, self.w2_s, rows.counts,
+                          rows.offsets, out=self.expert_y[:n], status=self.gemm_status,
+                          expected_rows=expect)
+        unpermute_tokens(self.expert_y[:n], rows, weights, out=out)
+        self.counts = rows.counts
+        return out
+
+    __call__ = forward
+
+    def dequantized_weights(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """fp32 views of this rank's weights as the kernels see them (for references)."""
+        return (self.w13_q.float() * self.w13_s.unsqueeze(-1),
+                self.w2_q.float() * self.w2_s.unsqueeze(-1))
+
+    def check_status(self) -> None:
+        if self.ata is not None:
+            self.ata.check_status()
+        if int(self.gemm_status.item()) != 0:
+            raise RuntimeError("pplx_kernels_b200: a grouped GEMM pipeline wait ran out")
+
+    def destroy(self) -> None:
+        if self.ata is not None:
+            self.ata.destroy()
+
+
+def moe_reference_int8(x: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor,
+                       w13: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
+    """Plain PyTorch statement of the int8 layer: activations pass through the same quantisation and
+    roundings as in the kernels, weights are given de-quantised."""
+    from ..ops.quant import quantize_rows_int8_reference
+
+    def through_int8(v: torch.Tensor) -> torch.Tensor:
+        q, scale = quantize_rows_int8_reference(v)
+        return q.to(torch.float32) * scale.unsqueeze(-1)
+
+    I = w2.size(2)
+    xq = through_int8(x)
+    out = torch.zeros(x.size(0), x.size(1), dtype=torch.float32, device=x.device)
+    idx = indices.to(torch.int64)
+    for k in range(idx.size(1)):
+        for e in idx[:, k].unique().tolist():
+            sel = (idx[:, k] == e).nonzero().flatten()
+            y = xq[sel] @ w13[e].t()
+            h = (torch.nn.functional.silu(y[:, :I]) * y[:, I:]).to(torch.bfloat16)
+            o = (through_int8(h) @ w2[e].t()).to(torch.bfloat16).to(torch.float32)
+            out[sel] += o * weights[sel, k : k + 1].to(torch.float32)
+    return out

@@ -3,6 +3,7 @@
     python -m pplx_kernels_b200.utils.bench_gemm --shape mixtral_up
     python -m pplx_kernels_b200.utils.bench_gemm --experts 8 --rows 512 --k 2048 --n 768 --swiglu
     python -m pplx_kernels_b200.utils.bench_gemm --shape mixtral_up --fp8
+    python -m pplx_kernels_b200.utils.bench_gemm --shape mixtral_up --int8
 
 Times with CUDA events after warm-up, flushing L2 between iterations; prints one
 JSON line with achieved TFLOP/s and the fraction of the measured bf16 peak
@@ -21,9 +22,10 @@ import torch
 from pplx_kernels_b200.ops.grouped_gemm import (
     grouped_gemm,
     grouped_gemm_fp8,
+    grouped_gemm_int8,
     quantize_weight_blocks,
 )
-from pplx_kernels_b200.ops.quant import per_token_block_quant
+from pplx_kernels_b200.ops.quant import per_token_block_quant, quantize_rows_int8
 
 SHAPES = {
     # name: (experts, rows per expert, K, N, swiglu)
@@ -54,7 +56,11 @@ def main() -> None:
                     help="block-scaled e4m3 kernel (with --swiglu its output is quantised too)")
     ap.add_argument("--pow2", action="store_true",
                     help="with --fp8: power-of-two scales, applied by the tensor cores")
+    ap.add_argument("--int8", action="store_true",
+                    help="8-bit integer kernel, a scale per token and per channel")
     args = ap.parse_args()
+    if args.int8 and args.fp8:
+        ap.error("--int8 or --fp8")
     if args.shape:
         E, rows, K, N, swiglu = SHAPES[args.shape]
     else:
@@ -85,6 +91,13 @@ def main() -> None:
         def ours():
             grouped_gemm_fp8(xq, sa, wq, sw, counts, swiglu_quant=swiglu, out=out8,
                              out_scale=out8_scale, status=status, pow2_scales=args.pow2)
+    elif args.int8:
+        xi, sx = quantize_rows_int8(x)
+        wi, sw = quantize_rows_int8(w)
+
+        def ours():
+            grouped_gemm_int8(xi, sx, wi, sw, counts, swiglu=swiglu, out=out, status=status,
+                              expected_rows=E * rows)
     else:
         def ours():
             grouped_gemm(x, w, counts, out=out, swiglu=swiglu, status=status,
@@ -117,7 +130,8 @@ def main() -> None:
     print(json.dumps({
         "shape": {"experts": E, "rows": rows, "k": K, "n": N, "swiglu": swiglu},
         "dtype": ("fp8_e4m3, power-of-two block scales in hardware" if args.fp8 and args.pow2
-                  else "fp8_e4m3 block-scaled" if args.fp8 else "bf16"),
+                  else "fp8_e4m3 block-scaled" if args.fp8
+                  else "int8, a scale per token and channel" if args.int8 else "bf16"),
         "us_p50": results["ours"],
         "tflops": tf,
         "frac_of_measured_bf16_peak": tf / peak if peak else None,

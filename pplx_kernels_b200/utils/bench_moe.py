@@ -26,8 +26,10 @@ from pplx_kernels_b200.models.configs import CONFIGS
 from pplx_kernels_b200.models.moe import (
     MoELayer,
     MoELayerFP8,
+    MoELayerInt8,
     moe_reference,
     moe_reference_fp8,
+    moe_reference_int8,
 )
 from pplx_kernels_b200.utils.testing import as_index_tensor, routing
 
@@ -63,6 +65,13 @@ def _fp8_layer(cfg, **kw):
     return MoELayerFP8(cfg, pow2_scales=POW2_SCALES, **kw)
 
 
+def _variants(layer) -> tuple:
+    """Names of a layer's forms and what selects them (the int8 layer is a composition only)."""
+    if isinstance(layer, MoELayerInt8):
+        return (("composed", {}),)
+    return ("composed", {"fused": False}), ("fused", {"fused": True})
+
+
 def verify_layer(layer, fp8: bool, x: torch.Tensor, idx: torch.Tensor, w: torch.Tensor,
                  world: int) -> str:
     """Runs the layer composed and fused and compares both with the reference.  Returns how it
@@ -72,8 +81,8 @@ def verify_layer(layer, fp8: bool, x: torch.Tensor, idx: torch.Tensor, w: torch.
     idx_dev = as_index_tensor(idx, dev)
     m = x.size(0)
     outs = {}
-    for name, fused in (("composed", False), ("fused", True)):
-        outs[name] = layer(x, idx_dev, w, fused=fused)[:m].float().clone()
+    for name, how in _variants(layer):
+        outs[name] = layer(x, idx_dev, w, **how)[:m].float().clone()
         torch.cuda.synchronize()
         layer.check_status()
     params = cfg.num_experts * 3 * cfg.hidden_dim * cfg.intermediate_dim
@@ -86,6 +95,13 @@ def verify_layer(layer, fp8: bool, x: torch.Tensor, idx: torch.Tensor, w: torch.
             f"{what}: largest error {float(err.max()):.4g} where {float(bound[err.argmax()] if err.dim() == 1 else bound.flatten()[err.argmax()]):.4g} "
             f"is allowed (largest value {float(want.abs().amax()):.4g})")
 
+    if isinstance(layer, MoELayerInt8):
+        if params > VERIFY_MAX_PARAMS:
+            return "not checked (the model is too large to gather for the reference)"
+        w13, w2 = layer.dequantized_weights()
+        want = moe_reference_int8(x, idx.to(dev), w, _gather(w13, world), _gather(w2, world))
+        close(outs["composed"], want, 3e-2, 2e-2, "against the int8 reference")
+        return "against the PyTorch reference over all experts"
     # The two paths do the same arithmetic; they may differ by roundings of the top-k sums only.
     close(outs["fused"], outs["composed"], 2e-2, 5e-3, "fused against composed")
     if params > VERIFY_MAX_PARAMS:
@@ -106,13 +122,13 @@ def verify_layer(layer, fp8: bool, x: torch.Tensor, idx: torch.Tensor, w: torch.
 def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: int,
             dev: torch.device, zipf: float = 0.0, graph: bool = False,
             flush: torch.Tensor | None = None, fp8: bool = False, replays: int = 1,
-            verify: bool = True) -> dict:
+            verify: bool = True, int8: bool = False) -> dict:
     """Times the MoE layer of `model` at `tokens` per GPU, composed and fused.  With more than one
     rank torch.distributed must be initialised (NCCL for CUDA tensors).  With `graph` a forward
     pass is captured once and every timed sample is `replays` back-to-back replays."""
     cfg = CONFIGS[model]
     m = tokens
-    make = _fp8_layer if fp8 else MoELayer
+    make = MoELayerInt8 if int8 else _fp8_layer if fp8 else MoELayer
     layer = make(cfg, max_num_tokens=m, rank=rank, world_size=world, device=dev)
     if world > 1:
         torch.distributed.barrier()  # weight initialisation takes a different time per rank
@@ -131,16 +147,16 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
             torch.distributed.barrier()
 
     res = {}
-    for name, fused in (("composed", False), ("fused", True)):
+    for name, how in _variants(layer):
         cuda_graph = None
         if graph:
-            layer(x, idx, w, out=out, fused=fused)
+            layer(x, idx, w, out=out, **how)
             torch.cuda.synchronize()
             barrier()
             stream = torch.cuda.Stream()
             cuda_graph = torch.cuda.CUDAGraph()
             with torch.cuda.stream(stream), torch.cuda.graph(cuda_graph, stream=stream):
-                layer(x, idx, w, out=out, fused=fused)
+                layer(x, idx, w, out=out, **how)
         times = []
         for it in range(warmup + iters):
             flush.add_(1)
@@ -152,7 +168,7 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
                 if cuda_graph is not None:
                     cuda_graph.replay()
                 else:
-                    layer(x, idx, w, out=out, fused=fused)
+                    layer(x, idx, w, out=out, **how)
             e1.record()
             torch.cuda.synchronize()
             if it >= warmup:
@@ -163,6 +179,7 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
         res[name] = float(t.median())
     layer.check_status()
     layer.destroy()
+    res.setdefault("fused", res["composed"])  # (a layer with one form)
 
     peaks = _peaks()
     # Per GPU: rows = tokens * top-k (uniform routing, weak scaling)
@@ -170,16 +187,16 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
     flops = rows * 6 * cfg.hidden_dim * cfg.intermediate_dim
     nle = cfg.num_experts // world
     # Weights that must stream from HBM: every local expert at large batches, at most one
-    # expert per row at small ones; one byte per weight in fp8, two in bf16.
+    # expert per row at small ones; one byte per weight in fp8 and int8, two in bf16.
     touched = min(nle, rows)
-    weight_bytes = touched * 3 * cfg.hidden_dim * cfg.intermediate_dim * (1 if fp8 else 2)
+    weight_bytes = touched * 3 * cfg.hidden_dim * cfg.intermediate_dim * (1 if fp8 or int8 else 2)
     wire_bytes = rows * cfg.hidden_dim * (world - 1) / world  # bytes per element below
-    # The measured bf16 peak for both dtypes: it is the one GEMM peak measured on the box (the
-    # fp8 tensor pipe is nominally twice as fast, so an fp8 layer can exceed this "floor").
+    # The measured bf16 peak for all dtypes: it is the one GEMM peak measured on the box (the
+    # 8-bit tensor pipes are nominally twice as fast, so such a layer can exceed this "floor").
     floors = {
         "compute_us": flops / (peaks["bf16_tflops"] * 1e6),
         "weights_hbm_us": weight_bytes / (peaks["hbm_gbs"] * 1e3),
-        "nvlink_dispatch_us": wire_bytes * (1 if fp8 else 2) / (NVLINK_GBS * 1e3),
+        "nvlink_dispatch_us": wire_bytes * (1 if fp8 or int8 else 2) / (NVLINK_GBS * 1e3),
         "nvlink_combine_us": wire_bytes * 2 / (NVLINK_GBS * 1e3),
     }
     floor = max(floors["compute_us"], floors["weights_hbm_us"],
@@ -188,7 +205,8 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
     return {
         "model": cfg.name,
         "dtype": ("fp8 block-scaled, power-of-two scales applied by the tensor cores"
-                  if fp8 and POW2_SCALES else "fp8 block-scaled" if fp8 else "bf16"),
+                  if fp8 and POW2_SCALES else "fp8 block-scaled" if fp8
+                  else "int8, a scale per token and channel" if int8 else "bf16"),
         "n_gpus": world,
         "tokens_per_gpu": m, "graph": graph, "replays_per_sample": replays if graph else 1,
         "zipf": zipf, "output_checked": checked,
@@ -290,11 +308,14 @@ def main() -> None:
     ap.add_argument("--fp8", action="store_true", help="block-scaled fp8 layer (MoELayerFP8)")
     ap.add_argument("--pow2", action="store_true",
                     help="with --fp8: power-of-two scales, applied by the tensor cores")
+    ap.add_argument("--int8", action="store_true", help="8-bit integer layer (MoELayerInt8)")
     ap.add_argument("--replays", type=int, default=1, help="graph replays per timed sample")
     ap.add_argument("--no-verify", action="store_true", help="skip the output check")
     ap.add_argument("--breakdown", action="store_true",
                     help="time each of the layer's four kernels instead of the layer")
     args = ap.parse_args()
+    if args.int8 and (args.fp8 or args.breakdown):
+        ap.error("--int8 goes with neither --fp8 nor --breakdown")
     global POW2_SCALES
     POW2_SCALES = bool(args.fp8 and args.pow2)
 
@@ -313,7 +334,7 @@ def main() -> None:
                 print(json.dumps(row), flush=True)
             continue
         row = measure(args.model, tokens, args.iters, args.warmup, rank, world, dev, args.zipf,
-                      args.graph, flush, args.fp8, args.replays, not args.no_verify)
+                      args.graph, flush, args.fp8, args.replays, not args.no_verify, args.int8)
         if rank == 0:
             print(json.dumps(row), flush=True)
     if world > 1:
