@@ -126,11 +126,16 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
 
 // --------------------------------------------------------------------- helpers ----
 
-// A row that no entry of the routing has.
-__device__ __forceinline__ bool is_rest(const ExpertRowsView& v, int64_t row) {
-  if (v.capacity == 0) return row >= v.offsets[v.num_experts];
-  const int64_t e = row / v.capacity;
-  return e >= v.num_experts || row - e * v.capacity >= v.counts[e];
+// Rows that no entry of the routing has: candidates (all rows where there is a capacity, otherwise
+// those behind the last expert's), and the row of candidate i, or -1 if an entry has it.
+__device__ __forceinline__ int64_t rest_candidates(const ExpertRowsView& v) {
+  if (v.capacity > 0) return v.num_rows;
+  return v.num_rows - min(max(static_cast<int64_t>(v.offsets[v.num_experts]), int64_t{0}), v.num_rows);
+}
+__device__ __forceinline__ int64_t rest_row(const ExpertRowsView& v, int64_t candidates, int64_t i) {
+  if (v.capacity == 0) return v.num_rows - candidates + i;
+  const int64_t e = i / v.capacity;
+  return i - e * v.capacity >= v.counts[e] ? i : -1;
 }
 
 // Row of entry (t, k), or -1.
@@ -241,7 +246,8 @@ __global__ void __launch_bounds__(kThreads) permute_kernel(const PermuteCall c) 
   const int lane = threadIdx.x & 31;
   const int vecs = static_cast<int>(c.row_bytes / static_cast<int64_t>(sizeof(V)));
   const int pieces = ceil_div(vecs, 32 * kBatch);
-  const int64_t units = (r.num_tokens + (c.zero_rest ? r.num_rows : 0)) * static_cast<int64_t>(pieces);
+  const int64_t rest = c.zero_rest ? rest_candidates(r) : 0;
+  const int64_t units = (r.num_tokens + rest) * static_cast<int64_t>(pieces);
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); u < units;
        u += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t t = u / pieces;
@@ -254,7 +260,8 @@ __global__ void __launch_bounds__(kThreads) permute_kernel(const PermuteCall c) 
         if (col + 32 * b < vecs) dst[col + 32 * b] = v[b];
     };
     if (t >= r.num_tokens) {
-      if (is_rest(r, t - r.num_tokens)) store(t - r.num_tokens);
+      const int64_t row = rest_row(r, rest, t - r.num_tokens);
+      if (row >= 0) store(row);
       continue;
     }
     const V* src = reinterpret_cast<const V*>(static_cast<const uint8_t*>(c.x) + t * c.x_stride);
@@ -270,131 +277,151 @@ __global__ void __launch_bounds__(kThreads) permute_kernel(const PermuteCall c) 
 
 // ------------------------------------------------------------------- unpermute ----
 
-// A warp per (token, piece of 32 vectors).
-template <typename T, int kVec>
+// A warp per (token, piece of its columns).  A lane has eight vectors in flight: kCols columns of
+// kRows rows.  4095 tokens of 8 rows of 7168 bf16: 84 us, 6.3 TB/s.
+template <typename T, int kVec, int kRows>
 __global__ void __launch_bounds__(kThreads) unpermute_kernel(const UnpermuteCall c) {
-  constexpr int kBatch = 8;  // rows whose vectors a lane has in flight
+  constexpr int kCols = 8 / kRows;
   using V = Vec<T, kVec>;
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   const int lane = threadIdx.x & 31;
   const int vecs = c.hidden / kVec;
-  const int pieces = ceil_div(vecs, 32);
+  const int pieces = ceil_div(vecs, 32 * kCols);
   int64_t tokens = r.num_tokens;
   if (c.bound_m != nullptr) tokens = min(tokens, static_cast<int64_t>(*c.bound_m));
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
        u < tokens * pieces; u += static_cast<int64_t>(gridDim.x) * kWarps) {
     const int64_t t = u / pieces;
-    const int col = static_cast<int>(u - t * pieces) * 32 + lane;
-    float sum[kVec] = {};
-    for (int k0 = 0; k0 < r.topk; k0 += kBatch) {
+    const int col = static_cast<int>(u - t * pieces) * 32 * kCols + lane;
+    float sum[kCols][kVec] = {};
+    for (int k0 = 0; k0 < r.topk; k0 += kRows) {
       // Lane k holds entry k0 + k.
       int my_row = -1;
       float my_w = 0.0f;
-      if (lane < kBatch && k0 + lane < r.topk) {
+      if (lane < kRows && k0 + lane < r.topk) {
         my_row = row_at(r, t, k0 + lane);
         my_w = my_row < 0 ? 0.0f : c.weights != nullptr ? c.weights[t * r.topk + k0 + lane] : 1.0f;
       }
-      V v[kBatch];
+      V v[kRows][kCols];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
+      for (int b = 0; b < kRows; ++b) {
         const int row = __shfl_sync(kAll, my_row, b);
-        v[b].clear();
-        if (row >= 0 && col < vecs)
-          v[b].load_once(static_cast<const T*>(c.y) + static_cast<int64_t>(row) * c.hidden, col);
+        const T* y = static_cast<const T*>(c.y) + static_cast<int64_t>(row) * c.hidden;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          v[b][i].clear();
+          if (row >= 0 && col + 32 * i < vecs) v[b][i].load_once(y, col + 32 * i);
+        }
       }
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
+      for (int b = 0; b < kRows; ++b) {
         const float w = __shfl_sync(kAll, my_w, b);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) sum[j] = fmaf(w, v[b].get(j), sum[j]);
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) sum[i][j] = fmaf(w, v[b][i].get(j), sum[i][j]);
       }
     }
-    if (col >= vecs) continue;
-    V o;
-    o.put(sum);
-    o.store(static_cast<T*>(c.out) + t * c.out_stride, col);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      V o;
+      o.put(sum[i]);
+      if (col + 32 * i < vecs) o.store(static_cast<T*>(c.out) + t * c.out_stride, col + 32 * i);
+    }
   }
 }
 
 // A block per token; behind the tokens, a block per row to be cleared.
-template <typename T, int kVec>
+template <typename T, int kVec, int kRows, int kCols>
 __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const UnpermuteBackwardCall c) {
-  constexpr int kBatch = 8;
   using V = Vec<T, kVec>;
-  __shared__ float part[kBatch][kWarps];
+  __shared__ float part[kRows][kWarps];
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   const int vecs = c.hidden / kVec;
   auto row_ptr = [&](auto* base, int64_t row) { return base + row * c.hidden; };
-  const int64_t blocks = r.num_tokens + (c.grad_y != nullptr ? r.num_rows : 0);
+  const int64_t rest = c.grad_y != nullptr ? rest_candidates(r) : 0;
+  const int64_t blocks = r.num_tokens + rest;
   for (int64_t t = blockIdx.x; t < blocks; t += gridDim.x) {
     if (t >= r.num_tokens) {
-      const int64_t row = t - r.num_tokens;
+      const int64_t row = rest_row(r, rest, t - r.num_tokens);
       V zero;
       zero.clear();
-      if (is_rest(r, row))
+      if (row >= 0)
         for (int col = tid; col < vecs; col += threads)
           zero.store(row_ptr(static_cast<T*>(c.grad_y), row), col);
       continue;
     }
     const T* grad = static_cast<const T*>(c.grad) + t * c.grad_stride;
-    for (int k0 = 0; k0 < r.topk; k0 += kBatch) {
+    for (int k0 = 0; k0 < r.topk; k0 += kRows) {
       // Lane k holds entry k0 + k.
       int my_row = -1;
       float my_w = 0.0f;
-      if (lane < kBatch && k0 + lane < r.topk) {
+      if (lane < kRows && k0 + lane < r.topk) {
         my_row = row_at(r, t, k0 + lane);
         my_w = c.weights[t * r.topk + k0 + lane];
       }
-      float dot[kBatch] = {};
-      for (int col0 = 0; col0 < vecs; col0 += threads) {
-        const int col = col0 + tid;
-        const bool in = col < vecs;
-        V g, y[kBatch];
-        g.clear();
-        if (in) g.load(grad, col);
+      float dot[kRows] = {};
+      for (int first = 0; first < vecs; first += threads * kCols) {  // (the same for all threads)
+        const int col0 = first + tid;
+        V g[kCols], y[kRows][kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          g[i].clear();
+          if (col0 + i * threads < vecs) g[i].load(grad, col0 + i * threads);
+        }
         if (c.grad_weights != nullptr) {
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
+          for (int b = 0; b < kRows; ++b) {
             const int row = __shfl_sync(kAll, my_row, b);
-            y[b].clear();
-            if (row >= 0 && in) y[b].load_once(row_ptr(static_cast<const T*>(c.y), row), col);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+              const int col = col0 + i * threads;
+              y[b][i].clear();
+              if (row >= 0 && col < vecs) y[b][i].load_once(row_ptr(static_cast<const T*>(c.y), row), col);
+            }
           }
         }
         if (c.grad_y != nullptr) {
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
+          for (int b = 0; b < kRows; ++b) {
             const int row = __shfl_sync(kAll, my_row, b);
             const float w = __shfl_sync(kAll, my_w, b);
-            float v[kVec];
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) v[j] = w * g.get(j);
-            V o;
-            o.put(v);
-            if (row >= 0 && in) o.store(row_ptr(static_cast<T*>(c.grad_y), row), col);
+            for (int i = 0; i < kCols; ++i) {
+              const int col = col0 + i * threads;
+              float v[kVec];
+#pragma unroll
+              for (int j = 0; j < kVec; ++j) v[j] = w * g[i].get(j);
+              V o;
+              o.put(v);
+              if (row >= 0 && col < vecs) o.store(row_ptr(static_cast<T*>(c.grad_y), row), col);
+            }
           }
         }
         if (c.grad_weights != nullptr) {
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b)
+          for (int b = 0; b < kRows; ++b)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) dot[b] = fmaf(y[b].get(j), g.get(j), dot[b]);
+            for (int i = 0; i < kCols; ++i)
+#pragma unroll
+              for (int j = 0; j < kVec; ++j) dot[b] = fmaf(y[b][i].get(j), g[i].get(j), dot[b]);
         }
       }
       if (c.grad_weights == nullptr) continue;
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
+      for (int b = 0; b < kRows; ++b) {
         float s = dot[b];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
         if (lane == 0) part[b][warp] = s;
       }
       __syncthreads();
-      if (tid < kBatch && k0 + tid < r.topk) {
+      if (tid < kRows && k0 + tid < r.topk) {
         float s = 0.0f;
         for (int w2 = 0; w2 < threads / 32; ++w2) s += part[tid][w2];
         c.grad_weights[t * r.topk + k0 + tid] = s;
@@ -440,13 +467,14 @@ __global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
   const int teams = kWarpTeam ? blockDim.x >> 5 : 1;
   const int vecs = c.hidden / kVec;
   const int64_t sources = kPermuted ? r.num_tokens : c.num_rows;
-  const int64_t items = sources + (c.zero_rest ? r.num_rows : 0);
+  const int64_t rest = c.zero_rest ? rest_candidates(r) : 0;
+  const int64_t items = sources + rest;
   int turn = 0;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * teams + (kWarpTeam ? warp : 0); t < items;
        t += static_cast<int64_t>(gridDim.x) * teams) {
     if (t >= sources) {
-      const int64_t row = t - sources;
-      if (!is_rest(r, row)) continue;
+      const int64_t row = rest_row(r, rest, t - sources);
+      if (row < 0) continue;
       Q zero;
       zero.clear();
       for (int col = tid; col < vecs; col += threads) zero.store(c.q + row * c.hidden, col);
@@ -548,9 +576,10 @@ uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 // Twice the blocks that fill every SM with 2048 threads; they loop over the rest.  (Once or four
 // times as many: 4096 x 28672 floats quantised in 103, 90, 90 us for once, twice, four times; copies of
 // 4096 tokens of 2048 25.0, 23.2, 24.5 us; the gradients of 4095 x 8 rows of 7168 170, 165, 164 us; their
-// sum 90, 91, 92 us.)
+// sum 90, 91, 92 us.  Once for small blocks: 8168 rows of 2048 bf16, 64 threads each, 8.7 and 10.8 us.)
 unsigned blocks_for(int64_t wanted, int threads) {
-  const int64_t most = static_cast<int64_t>(get_sm_count()) * std::min(32, 2048 / threads) * 2;
+  const int64_t most = static_cast<int64_t>(get_sm_count()) * std::min(32, 2048 / threads) *
+                       (threads < 128 ? 1 : 2);
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(wanted, most)));
 }
 
@@ -626,9 +655,16 @@ void launch_unpermute_tokens(const UnpermuteCall& c, cudaStream_t stream) {
   const uint64_t size = size_of(c.type);
   const int vec = alignment(16, {address(c.y), address(c.out), c.hidden * size, c.out_stride * size});
   with_type(c.type, vec, [&](auto t, auto v) {
-    const int64_t pieces = ceil_div<int64_t>(c.hidden / v.value, 32);
-    launch(unpermute_kernel<decltype(t), v.value>, c,
-           ceil_div<int64_t>(c.rows.num_tokens * pieces, kWarps), stream);
+    using T = decltype(t);
+    auto run = [&](auto* kernel, int cols) {
+      const int64_t pieces = ceil_div<int64_t>(c.hidden / v.value, 32 * cols);
+      launch(kernel, c, ceil_div<int64_t>(c.rows.num_tokens * pieces, kWarps), stream);
+    };
+    // us for 2, 4 and 8 rows at a time: 4096 tokens of 4096 bf16, top-2 18.6 / 18.7 / 41.4, top-1 13.0 /
+    // 16.5 / 32.7, top-4 29.2 / 25.3 / 45.1; of 2048, top-6 21.8 / 20.7 / 24.9; 4095 of 7168, top-8 93.4 /
+    // 83.5 / 95.3; 16 of 2048, top-8 4.2 / 3.0 / 2.7.
+    if (c.rows.topk <= 2) run(unpermute_kernel<T, v.value, 2>, 4);
+    else run(unpermute_kernel<T, v.value, 4>, 2);
   });
 }
 
@@ -639,11 +675,16 @@ void launch_unpermute_backward(const UnpermuteBackwardCall& c, cudaStream_t stre
   const int vec = alignment(16, {address(c.y), address(c.grad), address(c.grad_y), c.hidden * size,
                                  c.grad_stride * size});
   with_type(c.type, vec, [&](auto t, auto v) {
+    using T = decltype(t);
+    // us for 2 rows x 2 columns, 2 x 4, 4 x 1, 8 x 1: 4096 tokens of 4096 bf16, top-2 28.3, 30.0, 34.1, 50.3;
+    // top-4 50.8, 51.4, 50.2, 60.5; of 2048, top-6 38.2, 38.2, 42.9, 42.5; 4095 of 7168, top-8 159, 172,
+    // 161, 160; 16 of 2048, top-8 4.9, 5.0, 3.7, 3.4.
+    constexpr int kRows = 2, kCols = 2;
     // As few threads as cover a token's vectors in whole turns of the block.
     const int vecs = c.hidden / v.value;
-    const int turns = std::max(1, ceil_div(vecs, kThreads));
-    const int threads = std::min(kThreads, std::max(32, round_up(ceil_div(vecs, turns), 32)));
-    launch(unpermute_backward_kernel<decltype(t), v.value>, c, blocks, stream, threads);
+    const int turns = std::max(1, ceil_div(vecs, kThreads * kCols));
+    const int threads = std::min(kThreads, std::max(32, round_up(ceil_div(vecs, turns * kCols), 32)));
+    launch(unpermute_backward_kernel<T, v.value, kRows, kCols>, c, blocks, stream, threads);
   });
 }
 

@@ -61,7 +61,9 @@ class _LazyOps:
         return _LazyOps._namespace
 
     def __getattr__(self, name: str) -> object:
-        return getattr(self._resolve(), name)
+        op = getattr(self._resolve(), name)
+        self.__dict__[name] = op  # the next use finds it at once
+        return op
 
 
 _ops = _LazyOps()
