@@ -522,8 +522,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
       Q o;
 #pragma unroll
       for (int j = 0; j < kVec; j += 4)
-        o.w[j >> 2] = keep & quantize(v.get(j), kVec > 1 ? v.get(min(j + 1, kVec - 1)) : 0.0f,
-                                      kVec > 2 ? v.get(min(j + 2, kVec - 1)) : 0.0f,
+        o.w[j >> 2] = keep & quantize(v.get(j), v.get(j + 1), kVec > 2 ? v.get(min(j + 2, kVec - 1)) : 0.0f,
                                       kVec > 2 ? v.get(min(j + 3, kVec - 1)) : 0.0f, inv);
       return o;
     };
@@ -558,6 +557,86 @@ __global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
     for (int k = 0; k < targets; ++k) {
       const int64_t row = row_to(k);
       if (row >= 0 && tid == 0) c.scale[row] = scale;
+    }
+  }
+}
+
+// The same for rows that are not vectors of four: a block per token (or row of x), four values per
+// thread and turn, read one by one and (after the search for the largest) from the caches.  A row of q
+// may begin at any byte: a thread stores the aligned word that its values and those of the lane below
+// make up, and the ends of the row one byte at a time.
+template <typename T, bool kPermuted>
+__global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const QuantizeRowsCall c,
+                                                                   const ExpertRowsView r) {
+  using V = Vec<T, 1>;
+  __shared__ uint32_t part[2][kWarps];
+  ptx::wait_for_previous_kernels();
+  ptx::let_next_kernel_start();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t sources = kPermuted ? r.num_tokens : c.num_rows;
+  const int64_t rest = c.zero_rest ? rest_candidates(r) : 0;
+  int turn = 0;
+  for (int64_t t = blockIdx.x; t < sources + rest; t += gridDim.x) {
+    if (t >= sources) {
+      const int64_t row = rest_row(r, rest, t - sources);
+      if (row < 0) continue;
+      for (int col = tid; col < c.hidden; col += kThreads) c.q[row * c.hidden + col] = 0;
+      if (tid == 0) c.scale[row] = 0.0f;
+      continue;
+    }
+    if (!kPermuted && c.counts != nullptr) {
+      const int64_t plane = t / c.plane_rows;
+      if (t - plane * c.plane_rows >= c.counts[plane]) continue;
+    }
+    const T* x = static_cast<const T*>(c.x) + t * c.x_stride;
+    auto value = [&](int col) {
+      V v;
+      v.clear();
+      if (col < c.hidden) v.load(x, col);
+      return v.get(0);
+    };
+    uint32_t bits = 0;
+    for (int col = tid; col < c.hidden; col += 4 * kThreads)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits = max(bits, magnitude(value(col + i * kThreads)));
+    bits = __reduce_max_sync(kAll, bits);
+    if (lane == 0) part[turn][warp] = bits;
+    __syncthreads();
+    bits = __reduce_max_sync(kAll, lane < kWarps ? part[turn][lane] : 0u);
+    turn ^= 1;  // (the next row's maxima go elsewhere, so one barrier is enough)
+    const float amax = row_amax(bits);
+    const float inv = 127.0f / amax, scale = amax / 127.0f;
+    const uint32_t keep = amax < __uint_as_float(0x7f800000u) ? 0xffffffffu : 0u;
+    const int targets = kPermuted ? r.topk : 1;
+    int my_row = -1;  // lane k holds that of entry k
+    if (kPermuted && lane < r.topk) my_row = row_at(r, t, lane);
+    // A warp makes 32 words and stores 31: the lowest lane only hands its values up.  (The last word of
+    // a row that begins inside one is behind the row's last values.)
+    for (int turn_of = warp; turn_of * 31 * 4 < c.hidden + 4; turn_of += kWarps) {
+      const int col = (turn_of * 31 + lane - 1) * 4;
+      uint32_t word = 0;
+      if (col >= 0) word = keep & quantize(value(col), value(col + 1), value(col + 2), value(col + 3), inv);
+      const uint32_t below = __shfl_up_sync(kAll, word, 1);
+      for (int k = 0; k < targets; ++k) {
+        int64_t row = t;
+        if constexpr (kPermuted) row = k < 32 ? __shfl_sync(kAll, my_row, k) : row_at(r, t, k);
+        if (row < 0 || lane == 0) continue;
+        int8_t* q = c.q + row * c.hidden;
+        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(q) & 3u);
+        const uint32_t out = __funnelshift_l(below, word, 8 * shift);
+        const int at = col - shift;  // of the first byte of `out`
+        if (at >= 0 && at + 4 <= c.hidden) {
+          *reinterpret_cast<uint32_t*>(q + at) = out;
+        } else {
+#pragma unroll 1
+          for (int j = max(0, -at); j < min(4, c.hidden - at); ++j)
+            q[at + j] = static_cast<int8_t>(out >> (8 * j));
+        }
+      }
+    }
+    for (int k = tid; k < targets; k += kThreads) {
+      const int64_t row = kPermuted ? row_at(r, t, k) : t;
+      if (row >= 0) c.scale[row] = scale;
     }
   }
 }
@@ -710,12 +789,16 @@ void launch_quantize_rows(const QuantizeRowsCall& c, cudaStream_t stream) {
     };
     auto pick = [&](auto permuted) {
       constexpr bool kPermuted = decltype(permuted)::value;
-      if (vecs <= 32 * 4)
-        return run(quantize_kernel<T, v.value, 4, true, kPermuted>, kThreads, ceil_div<int64_t>(items, kWarps));
-      if (vecs <= kThreads * 4)
-        return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32), items);
-      const int threads = std::min(kThreads, round_up(ceil_div(vecs, 8), 32));
-      run(quantize_kernel<T, v.value, 8, false, kPermuted>, threads, items);
+      if constexpr (v.value == 1) {
+        run(quantize_ragged_kernel<T, kPermuted>, kThreads, items);
+      } else {
+        if (vecs <= 32 * 4)
+          return run(quantize_kernel<T, v.value, 4, true, kPermuted>, kThreads, ceil_div<int64_t>(items, kWarps));
+        if (vecs <= kThreads * 4)
+          return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32), items);
+        const int threads = std::min(kThreads, round_up(ceil_div(vecs, 8), 32));
+        run(quantize_kernel<T, v.value, 8, false, kPermuted>, threads, items);
+      }
     };
     if (c.rows != nullptr) pick(std::true_type{});
     else pick(std::false_type{});
