@@ -613,17 +613,17 @@ void launch_one(const CUtensorMap& tmap_w, const TokenMaps& tmap_x, Int8GemmArgs
 }
 
 // Single CTAs, whose tiles of 128 weight rows divide a launch more finely, up to an expected mean of
-// 112 rows per expert; pairs, which read the tokens half as often, from there on.  us, single and
-// pairs: 128 experts of 768 x 2048, up projection 2 rows 65.1 / 68.8, 64 rows 70.7 / 76.8, 128 rows
-// 78.0 / 81.1, 256 rows 98.5 / 92.4; 32 experts of 2048 x 7168, up 8 rows 143.0 / 141.4, 128 rows
-// 153.7 / 150.7, 256 rows 198 / 176; down 64 rows 81.0 / 84.3, 128 rows 89.1 / 88.3, 256 rows 116.5 /
-// 104.9.
+// 64 rows per expert; pairs, which read the tokens half as often, from there on.  us, single and pairs,
+// up projection: 128 experts of 768 x 2048, 8000 rows evenly 71.3 / 75.4, with a popularity of exponent
+// 0.6 76.7 / 74.1, 1.2 81.3 / 80.1, 16000 rows 80.1 / 78.6, 90.3 / 85.7, 95.8 / 90.1; 64 experts of 1408
+// x 2048, 1800 rows 62.6 / 64.9, 64.6 / 63.2, 68.2 / 65.0, 6000 rows 69.7 / 69.2, 75.9 / 71.8, 81.1 /
+// 76.8; 32 experts of 2048 x 7168, 8000 rows 232 / 195, 232 / 211, 244 / 231.
 bool want_pairs(const Int8GemmCall& c) {
   const int64_t rows = c.expected_total_rows > 0 ? c.expected_total_rows
                        : c.offsets != nullptr
                            ? c.rows_per_expert
                            : static_cast<int64_t>(c.num_experts) * c.rows_per_expert;
-  return rows > 112 * static_cast<int64_t>(c.num_experts);
+  return rows > 64 * static_cast<int64_t>(c.num_experts);
 }
 
 template <bool SWIGLU>
