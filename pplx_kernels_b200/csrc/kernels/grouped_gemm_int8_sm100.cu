@@ -92,6 +92,7 @@ struct Control {
   uint32_t max_width;
   unsigned long long best_limit;
   Tile tiles[kTable];
+  uint32_t warp_tiles[kThreads / 32];
   alignas(128) uint8_t seg[8][32 * 64];  // of each epilogue warp: 32 tokens' columns
   alignas(16) float sx[2][kMaxTokens];  // scales of a tile's tokens, of two tiles in turn
 };
@@ -173,8 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   __syncthreads();
-  for (int e = tid; e < g.num_experts; e += blockDim.x) {
-    // (Counts and offsets that do not fit the tensors are cut to them.)
+  // (Counts and offsets that do not fit the tensors are cut to them.)
+  auto read_rows = [&](int e) {
     int first = 0, most = g.rows_per_expert;
     if (g.offsets != nullptr) {
       first = min(max(g.offsets[e], 0), g.rows_per_expert);
@@ -183,54 +184,94 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows = g.counts != nullptr ? min(max(g.counts[e], 0), most) : most;
     rows_of[e] = static_cast<uint32_t>(rows);
     row0_of[e] = static_cast<uint32_t>(first);
-    if (rows > 0) atomicMax(&ctl->max_rows, static_cast<uint32_t>(rows));
-  }
-  __syncthreads();
-  // The most token rows a tile may have.  One tile per expert up to 256 rows: there an expert is
-  // bound by its weights, which more tiles would only read again.  Above, the limit that
-  // minimises (waves of tiles) x (time of a tile).  Measured, in cycles per K block of 128 bytes of a
-  // tile of w rows: 330 + 5/3 w up to 256 rows, 220 + 11/5 w up to 384 and 18/5 w - 340 above (there
-  // are fewer stages); more than the 2 w cycles of its MMAs, because L2 delivers some 42 bytes per
-  // cycle and SM, of 16 KB of weights and 64 w bytes of tokens.  And the epilogue of more than 256 rows
-  // is not hidden as a whole: 6 cycles per row with three accumulators, 10 with two.  Every CTA computes
-  // the same.  (us for one tile of all rows and two of half of them: 32 experts of 2048 x 7168, up, 320
-  // rows each 206, 255; 384: 241, 283; 512: 308, 310; down 320 rows 130, 141; 512: 199, 171.)
+    return rows;
+  };
   int limit = kPair ? kMaxTokens : kMmaTokens;
-  if (ctl->max_rows > kMmaTokens) {
-    for (int cand = limit - kUnit * warp; 4 * cand >= limit; cand -= kUnit * (kThreads / 32)) {
-      uint32_t tiles = 0, width = 0;
-      for (int e = lane; e < g.num_experts; e += 32) {
-        const Cut<kUnit> cut(static_cast<int>(rows_of[e]), cand);
-        tiles += cut.tiles;
-        width += cut.units * kUnit;
-      }
-      tiles = __reduce_add_sync(0xffffffffu, tiles);
-      width = __reduce_add_sync(0xffffffffu, width);
-      if (lane == 0) {
-        const uint64_t waves = ceil_div<uint64_t>(static_cast<uint64_t>(tiles) * w_blocks, workers);
-        const uint32_t w = width / tiles;
-        const uint64_t each = max(max(330u + 5u * w / 3u, 220u + 11u * w / 5u), 18u * max(w, 100u) / 5u - 340u);
-        const uint32_t drain = cand <= kMmaTokens ? 0u : cand <= 2 * kThirdCols ? 6u : 10u;
-        const uint64_t cost = waves * (num_kb * each + drain * w);
-        atomicMin(&ctl->best_limit, (cost << 16) | static_cast<uint64_t>(kMaxTokens - cand));
-      }
+  uint32_t total_tiles, max_width;
+  // One expert per thread, and none with more than one token tile: everything by two block barriers
+  // (24 rows through 128 experts of 2048 x 768: 8.6 us, 9.3 the long way).
+  const int my_rows = tid < g.num_experts ? read_rows(tid) : 0;
+  for (int e = tid + kThreads; e < g.num_experts; e += kThreads) atomicMax(&ctl->max_rows, read_rows(e));
+  {
+    const uint32_t mine = my_rows > 0 ? w_blocks : 0;
+    const uint32_t upto = warp_inclusive_scan(mine, lane);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(my_rows));
+    if (lane == 31) {
+      ctl->warp_tiles[warp] = upto;
+      if (most > 0) atomicMax(&ctl->max_rows, most);
     }
     __syncthreads();
-    limit = kMaxTokens - static_cast<int>(ctl->best_limit & 0xffffu);
+    const uint32_t max_rows = ctl->max_rows;
+    if (max_rows <= kMmaTokens && g.num_experts <= kThreads) {
+      uint32_t before = 0;
+      total_tiles = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w == warp) before = total_tiles;
+        total_tiles += ctl->warp_tiles[w];
+      }
+      max_width = max(round_up<uint32_t>(max_rows, kUnit), static_cast<uint32_t>(kUnit));
+      const uint32_t start = before + upto - mine;
+      if (tid < g.num_experts) tile_start[tid] = start;
+      if (tid == 0) tile_start[g.num_experts] = total_tiles;
+      // This worker's tiles of the thread's expert, as far as they are among its first.
+      if (mine > 0)
+        for (uint32_t i = start > worker ? (start - worker + workers - 1) / workers : 0;
+             i < kTable && worker + i * workers < start + mine; ++i)
+          ctl->tiles[i] = {tid, static_cast<int>(worker + i * workers - start), 0,
+                           round_up(my_rows, kUnit), my_rows};
+    } else {
+      // The most token rows a tile may have.  One tile per expert up to 256 rows: there an expert is
+      // bound by its weights, which more tiles would only read again.  Above, the limit that
+      // minimises (waves of tiles) x (time of a tile).  Measured, in cycles per K block of 128 bytes
+      // of a tile of w rows: 330 + 5/3 w up to 256 rows, 220 + 11/5 w up to 384 and 18/5 w - 340 above
+      // (there are fewer stages); more than the 2 w cycles of its MMAs, because L2 delivers some 42
+      // bytes per cycle and SM, of 16 KB of weights and 64 w bytes of tokens.  And the epilogue of more
+      // than 256 rows is not hidden as a whole: 6 cycles per row with three accumulators, 10 with two.
+      // Every CTA computes the same.  (us for one tile of all rows and two of half of them: 32 experts
+      // of 2048 x 7168, up, 320 rows each 206, 255; 384: 241, 283; 512: 308, 310; down 320 rows 130,
+      // 141; 512: 199, 171.)
+      if (max_rows > kMmaTokens) {
+        for (int cand = limit - kUnit * warp; 4 * cand >= limit; cand -= kUnit * (kThreads / 32)) {
+          uint32_t tiles = 0, width = 0;
+          for (int e = lane; e < g.num_experts; e += 32) {
+            const Cut<kUnit> cut(static_cast<int>(rows_of[e]), cand);
+            tiles += cut.tiles;
+            width += cut.units * kUnit;
+          }
+          tiles = __reduce_add_sync(0xffffffffu, tiles);
+          width = __reduce_add_sync(0xffffffffu, width);
+          if (lane == 0) {
+            const uint64_t waves =
+                ceil_div<uint64_t>(static_cast<uint64_t>(tiles) * w_blocks, workers);
+            const uint32_t w = width / tiles;
+            const uint64_t each =
+                max(max(330u + 5u * w / 3u, 220u + 11u * w / 5u), 18u * max(w, 100u) / 5u - 340u);
+            const uint32_t drain = cand <= kMmaTokens ? 0u : cand <= 2 * kThirdCols ? 6u : 10u;
+            const uint64_t cost = waves * (num_kb * each + drain * w);
+            atomicMin(&ctl->best_limit, (cost << 16) | static_cast<uint64_t>(kMaxTokens - cand));
+          }
+        }
+        __syncthreads();
+        limit = kMaxTokens - static_cast<int>(ctl->best_limit & 0xffffu);
+      }
+      for (int e = tid; e < g.num_experts; e += kThreads) {
+        const Cut<kUnit> cut(static_cast<int>(rows_of[e]), limit);
+        tile_start[e] = static_cast<uint32_t>(cut.tiles * w_blocks);
+        if (cut.tiles > 0) atomicMax(&ctl->max_width, static_cast<uint32_t>(cut.widest()));
+      }
+      __syncthreads();
+      if (warp == 0) warp_exclusive_scan_smem(tile_start, g.num_experts, lane, true);
+      __syncthreads();
+      // The search for a tile takes one thread some 500 cycles: those of this worker's first tiles
+      // are made side by side.
+      total_tiles = tile_start[g.num_experts];
+      max_width = ctl->max_width;
+      if (tid < kTable && worker + tid * workers < total_tiles)
+        ctl->tiles[tid] =
+            locate<kUnit>(tile_start, rows_of, g.num_experts, limit, worker + tid * workers);
+    }
   }
-  for (int e = tid; e < g.num_experts; e += blockDim.x) {
-    const Cut<kUnit> cut(static_cast<int>(rows_of[e]), limit);
-    tile_start[e] = static_cast<uint32_t>(cut.tiles * w_blocks);
-    if (cut.tiles > 0) atomicMax(&ctl->max_width, static_cast<uint32_t>(cut.widest()));
-  }
-  __syncthreads();
-  if (warp == 0) warp_exclusive_scan_smem(tile_start, g.num_experts, lane, true);
-  __syncthreads();
-  // The search for a tile takes one thread some 500 cycles: those of this worker's first tiles are
-  // made side by side.
-  const uint32_t total_tiles = tile_start[g.num_experts];
-  if (tid < kTable && worker + tid * workers < total_tiles)
-    ctl->tiles[tid] = locate<kUnit>(tile_start, rows_of, g.num_experts, limit, worker + tid * workers);
   auto tile = [&](uint32_t local) {
     return local < kTable ? ctl->tiles[local]
                           : locate<kUnit>(tile_start, rows_of, g.num_experts, limit,
@@ -243,13 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
   // As many stages as the launch's widest token tile leaves room for.
-  const uint32_t stage_bytes = kWBytes + ctl->max_width / kCtas * kRowBytes;
+  const uint32_t stage_bytes = kWBytes + max_width / kCtas * kRowBytes;
   const uint32_t stages = min(g.ring_bytes / stage_bytes, static_cast<uint32_t>(kMaxStages));
   // Accumulators are slots of tensor memory that the MMAs take in turn: two of 256 columns, or three
   // of 160 where a tile is wider than 256 rows, but none than 320.  A tile that is wider than a slot is
   // two halves, each with its MMAs and a slot of its own, so that the MMAs of a tile can begin while
   // the second half (with three: both) of the tile before is read out.
-  const bool thirds = kPair && ctl->max_width > kMmaTokens && ctl->max_width <= 2 * kThirdCols;
+  const bool thirds = kPair && max_width > kMmaTokens && max_width <= 2 * kThirdCols;
   const int slot_cols = thirds ? kThirdCols : kMmaTokens;
   const uint32_t slots = thirds ? 3u : 2u;
   auto first_half = [&](int width) {
