@@ -70,6 +70,10 @@ int64_t token_stride(const at::Tensor& t, const char* op, const char* name) {
   return t.size(0) <= 1 ? t.size(1) : t.stride(0);
 }
 
+void check_hidden(int64_t hidden, const char* op) {
+  TORCH_CHECK(hidden < (int64_t{1} << 30), op, ": rows of 2^30 elements or more");
+}
+
 // Rows as the capacity says: [rows, hidden] or [experts, capacity, hidden], contiguous.
 void check_rows(const at::Tensor& t, const ExpertRowsView& v, int64_t hidden, const at::Tensor& like,
                 const char* op, const char* name) {
@@ -193,6 +197,7 @@ void permute_tokens_out_op(const at::Tensor& x, const at::Tensor& counts, const 
   c.rows = make_view(counts, offsets, row_of, capacity, x, op);
   c.x_stride = token_stride(x, op, "x") * x.element_size();
   TORCH_CHECK(x.size(0) == c.rows.num_tokens, op, ": x and row_of disagree on the token count");
+  check_hidden(x.size(1), op);
   check_rows(out, c.rows, x.size(1), x, op, "out");
   TORCH_CHECK(out.scalar_type() == x.scalar_type(), op, ": out must have the type of x");
   c.x = data<void>(x);
@@ -207,10 +212,6 @@ at::Tensor permute_tokens_op(const at::Tensor& x, const at::Tensor& counts, cons
   at::Tensor out = empty_rows(x, counts, row_of, capacity, x.scalar_type());
   permute_tokens_out_op(x, counts, offsets, row_of, capacity, out, zero_rest);
   return out;
-}
-
-void check_hidden(int64_t hidden, const char* op) {
-  TORCH_CHECK(hidden < (int64_t{1} << 30), op, ": rows of 2^30 elements or more");
 }
 
 void permute_tokens_int8_out_op(const at::Tensor& x, const at::Tensor& counts, const at::Tensor& offsets,

@@ -353,6 +353,59 @@ def test_streams_and_graphs():
     assert torch.equal(x.grad, want[1]) and torch.equal(w.grad, want[2])
 
 
+def test_captured_backward_with_leaves_of_its_own():
+    """Forward and backward captured as autograd records them, with leaves made in the capture, while an
+    eager graph of the tensors behind them lives."""
+    m, topk, experts, hidden = 24, 2, 4, 128
+    x, w = data(m, hidden).requires_grad_(), torch.rand(m, topk, device=DEV).requires_grad_()
+    g = data(m, hidden, seed=2)
+    idx = routing(m, topk, experts)
+
+    def step(x, w):
+        rows = sort_by_expert(idx, experts)
+        out = unpermute_tokens(torch.tanh(permute_tokens(x, rows)), rows, w)
+        out.backward(g)
+        return out.detach(), x.grad, w.grad
+
+    rows = sort_by_expert(idx, experts)
+    eager = unpermute_tokens(torch.tanh(permute_tokens(x, rows)), rows, w)  # lives until the end
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x.detach().requires_grad_(), w.detach().requires_grad_())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x.detach().requires_grad_(), w.detach().requires_grad_())
+    with torch.no_grad():
+        x.mul_(-0.5)
+    idx.copy_(routing(m, topk, experts, seed=9))
+    graph.replay()
+    want = step(x.detach().requires_grad_(), w.detach().requires_grad_())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert eager.shape == (m, hidden)
+
+
+def test_second_derivatives():
+    """The copy and the plain sum are linear, so their gradients have gradients; that of the weighted
+    sum is refused."""
+    m, topk, hidden = 6, 2, 32
+    rows = sort_by_expert(routing(m, topk, 4), 4)
+    x, y = data(m, hidden).requires_grad_(), data(m * topk, hidden, seed=2).requires_grad_()
+    g = data(m, hidden, seed=3).requires_grad_()
+    (gy,) = torch.autograd.grad(unpermute_tokens(y, rows), y, g, create_graph=True)
+    (gg,) = torch.autograd.grad(gy.sum(), g)
+    assert (gg == topk).all()
+    gr = data(m * topk, hidden, seed=4).requires_grad_()
+    (gx,) = torch.autograd.grad(permute_tokens(x, rows), x, gr, create_graph=True)
+    (gg,) = torch.autograd.grad(gx.sum(), gr)
+    assert (gg == 1).all()
+    w = torch.rand(m, topk, device=DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="no derivative of its own"):
+        torch.autograd.grad(unpermute_tokens(y, rows, w), w, g, create_graph=True)
+
+
 def test_rows_behind_four_gigabytes():
     """Offsets into the rows pass 32 bits."""
     m, topk, hidden = 70000, 8, 4096  # 4.6 GB of rows
