@@ -22,7 +22,7 @@ namespace pplx {
 namespace {
 
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr int kMaxSortExperts = 1024;
+constexpr int kMaxSortExperts = 1024;  // (their numbers and one more take 11 bits)
 
 // ------------------------------------------------------------------------ sort ----
 
@@ -30,8 +30,8 @@ constexpr int kSortThreads = 512;
 
 __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t cta) {
   uint32_t addr, v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tc::smem_u32(p)), "r"(cta));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tc::smem_u32(p)), "r"(cta));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
 
@@ -41,13 +41,15 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t cta) 
 // latency: of the entries' loads, the match of 32 entries, three block barriers.
 template <typename Index>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExpertCall c) {
+  constexpr int kHeld = 8;
   extern __shared__ uint32_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
   const int blocks = gridDim.x;
   const int E = c.num_experts;
   uint32_t* seen = smem;               // [warps][E]
   uint32_t* mine_all = smem + warps * E;  // [E] entries of this block
-  uint32_t* first = mine_all + E;      // [E + 1]
+  uint32_t* before_of = mine_all + E;  // [E] entries of the blocks before this one
+  uint32_t* first = before_of + E;     // [E + 1]
   for (int i = tid; i < warps * E; i += blockDim.x) seen[i] = 0;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
@@ -63,20 +65,45 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
   const int begin = static_cast<int>(min(static_cast<int64_t>(run) * per, static_cast<int64_t>(n)));
   const int end = min(begin + per, n);
   uint32_t* mine = seen + warp * E;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    int e = E;  // none
-    if (i < min(end, live)) {
-      const Index v = indices[i];
-      if (v < static_cast<Index>(E)) e = static_cast<int>(v);
+  const int bits = 32 - __clz(E);  // of the numbers 0 .. E
+  auto load_index = [&](int i) { return i < min(end, live) ? indices[i] : static_cast<Index>(E); };
+  auto expert_of = [&](Index v) { return v < static_cast<Index>(E) ? static_cast<int>(v) : E; };  // E: none
+  // How many entries of the run came before this lane's of the same expert.
+  auto count = [&](int e) {
+    // (A vote per bit of the expert's number; match.any took 0.6 us per 32 entries that differ.)
+    uint32_t same = kAll;
+#pragma unroll
+    for (int b = 0; b < 11; ++b) {
+      if (b >= bits) break;
+      const uint32_t set = __ballot_sync(kAll, (e >> b) & 1);
+      same &= (e >> b) & 1 ? set : ~set;
     }
-    const uint32_t same = __match_any_sync(kAll, e);
     const uint32_t before = __popc(same & ((1u << lane) - 1u));
     const uint32_t base = e < E ? mine[e] : 0u;
     __syncwarp();
     if (e < E && before == 0) mine[e] = base + __popc(same);
     __syncwarp();
-    if (i < end) c.row_of[i] = e < E ? static_cast<int32_t>(base + before) : -1;
+    return static_cast<int32_t>(base + before);
+  };
+  // Up to kHeld entries of a lane stay in registers; longer runs keep the numbers in row_of.
+  const bool held = per <= 32 * kHeld;
+  int expert[kHeld], local[kHeld];
+  if (held) {
+    Index v[kHeld];
+#pragma unroll
+    for (int s = 0; s < kHeld; ++s) v[s] = load_index(begin + 32 * s + lane);  // (all on their way)
+#pragma unroll
+    for (int s = 0; s < kHeld; ++s) {
+      if (32 * s >= per) break;
+      expert[s] = expert_of(v[s]);
+      local[s] = count(expert[s]);
+    }
+  } else {
+    for (int i0 = begin; i0 < end; i0 += 32) {
+      const int e = expert_of(load_index(i0 + lane));
+      const int32_t n_before = count(e);
+      if (i0 + lane < end) c.row_of[i0 + lane] = e < E ? n_before : -1;
+    }
   }
   __syncthreads();
   for (int e = tid; e < E; e += blockDim.x) {
@@ -89,17 +116,24 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
     mine_all[e] = sum;
     first[e] = sum;
   }
+  if (blocks == 1)
+    for (int e = tid; e < E; e += blockDim.x) before_of[e] = 0;
   if (blocks > 1) {
     tc::cluster_sync();
     for (int e = tid; e < E; e += blockDim.x) {
       uint32_t sum = 0, before = 0;
-      for (int b = 0; b < blocks; ++b) {
-        const uint32_t v = ld_cluster(&mine_all[e], b);
-        if (b == static_cast<int>(blockIdx.x)) before = sum;
-        sum += v;
+      for (int b0 = 0; b0 < blocks; b0 += 8) {  // (8 or 16 blocks)
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = ld_cluster(&mine_all[e], b0 + j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (b0 + j == static_cast<int>(blockIdx.x)) before = sum;
+          sum += v[j];
+        }
       }
       first[e] = sum;
-      for (int w = 0; w < warps; ++w) seen[w * E + e] += before;
+      before_of[e] = before;
     }
     tc::cluster_sync();  // (no block leaves while others read its sums)
   } else {
@@ -114,13 +148,22 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
   if (blockIdx.x == 0)
     for (int e = tid; e <= E; e += blockDim.x)
       c.offsets[e] = c.capacity > 0 ? e * c.capacity : static_cast<int>(first[e]);
-  for (int i = begin + lane; i < end; i += 32) {
-    const int32_t local = c.row_of[i];  // (of this thread)
-    if (local < 0) continue;
-    const int e = static_cast<int>(indices[i]);
-    const int pos = static_cast<int>(mine[e]) + local;
-    if (c.capacity > 0) c.row_of[i] = pos < c.capacity ? e * c.capacity + pos : -1;
-    else c.row_of[i] = static_cast<int>(first[e]) + pos;
+  auto row_of = [&](int e, int32_t n_before) -> int32_t {
+    const int pos = static_cast<int>(mine[e] + before_of[e]) + n_before;
+    if (c.capacity > 0) return pos < c.capacity ? e * c.capacity + pos : -1;
+    return static_cast<int>(first[e]) + pos;
+  };
+  if (held) {
+#pragma unroll
+    for (int s = 0; s < kHeld; ++s) {
+      const int i = begin + 32 * s + lane;
+      if (i < end) c.row_of[i] = expert[s] < E ? row_of(expert[s], local[s]) : -1;
+    }
+  } else {
+    for (int i = begin + lane; i < end; i += 32) {
+      const int32_t n_before = c.row_of[i];  // (written by this thread)
+      if (n_before >= 0) c.row_of[i] = row_of(static_cast<int>(indices[i]), n_before);
+    }
   }
 }
 
@@ -696,13 +739,13 @@ void launch_sort_by_expert(const SortByExpertCall& c, cudaStream_t stream) {
   auto* kernel = c.wide_indices ? sort_kernel<uint64_t> : sort_kernel<uint32_t>;
   const int64_t n = static_cast<int64_t>(c.num_tokens) * c.topk;
   // us with 256 experts, one block of 256 / 512 threads, clusters of 8 / 16 blocks of 512: 8 entries
-  // 2.8 / 3.0 / 4.7 / 5.3, 512 entries 3.9 / 3.7 / 5.2 / 5.9, 1024 entries 4.6 / 4.5 / 5.3 / 5.8, 4096
-  // entries 10.0 / 7.9 / 5.4 / 5.9, 8192 entries 17.0 / 12.9 / 6.1 / 5.9, 32768 entries 80 / 51 /
-  // 10.7 / 8.1.
+  // 3.0 / 3.3 / 4.3 / 4.9, 512 entries 3.7 / 3.6 / 4.3 / 4.9, 1024 entries 4.3 / 4.0 / 4.3 / 4.9, 2048
+  // entries 5.6 / 4.9 / 4.2 / 4.9, 8192 entries 20.3 / 13.5 / 4.9 / 5.0, 32768 entries 92.7 / 51.9 / 7.5 /
+  // 6.2.
   const int blocks = n <= 1024 ? 1 : n <= 8192 ? 8 : 16;
   const int threads = n <= 256 ? 256 : kSortThreads;
   const int warps = threads / 32;
-  const size_t smem = sizeof(uint32_t) * (static_cast<size_t>(warps + 2) * c.num_experts + 1);
+  const size_t smem = sizeof(uint32_t) * (static_cast<size_t>(warps + 3) * c.num_experts + 1);
   if (smem > 48 * 1024)
     CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(smem)));
