@@ -38,7 +38,8 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t cta) 
 // Warps take runs of entries.  A warp counts its entries per expert and remembers for each entry
 // how many of its expert came before it in the run; the runs' counts are then summed over the warps,
 // the blocks (one, or a cluster whose blocks read each other's sums) and the experts.  Bound by
-// latency: of the entries' loads, the match of 32 entries, three block barriers.
+// latency: of the entries' loads (up to eight of a lane at once), of the votes that find a warp's entries
+// of one expert, of the barriers.
 template <typename Index>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExpertCall c) {
   constexpr int kHeld = 8;
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortByExper
   auto expert_of = [&](Index v) { return v < static_cast<Index>(E) ? static_cast<int>(v) : E; };  // E: none
   // How many entries of the run came before this lane's of the same expert.
   auto count = [&](int e) {
-    // (A vote per bit of the expert's number; match.any took 0.6 us per 32 entries that differ.)
+    // (A vote per bit of the expert's number: 32768 entries 7.0 us, with match.any 7.6.)
     uint32_t same = kAll;
 #pragma unroll
     for (int b = 0; b < 11; ++b) {
