@@ -44,6 +44,7 @@ struct PermuteCall {
   void* out = nullptr;    // [num_rows] packed rows
   int64_t row_bytes = 0;
   bool zero_rest = false;
+  bool streaming = false;  // set by the launcher
 };
 void launch_permute_tokens(const PermuteCall& call, cudaStream_t stream);
 
@@ -58,6 +59,7 @@ struct UnpermuteCall {
   void* out = nullptr;
   int64_t out_stride = 0;              // elements
   int hidden = 0;
+  bool streaming = false;              // set by the launcher
 };
 void launch_unpermute_tokens(const UnpermuteCall& call, cudaStream_t stream);
 
@@ -92,6 +94,7 @@ struct QuantizeRowsCall {
   int8_t* q = nullptr;    // packed rows
   float* scale = nullptr;
   int hidden = 0;
+  bool streaming = false;  // set by the launcher
 };
 void launch_quantize_rows(const QuantizeRowsCall& call, cudaStream_t stream);
 

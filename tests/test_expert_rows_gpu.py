@@ -106,7 +106,10 @@ def test_permute(dtype, hidden, capacity):
         permute_tokens(x, rows, out=out)
         token = token_of(rows, total)
         there = (token >= 0).view(*rows.shape(), 1)
-        as_bytes = lambda t: t.contiguous().view(torch.uint8)
+
+        def as_bytes(t):
+            return t.contiguous().view(torch.uint8)
+
         size = dtype.itemsize
         want = as_bytes(x)[token.clamp(min=0)].view(*rows.shape(), hidden * size)
         assert torch.equal(as_bytes(out), torch.where(there, want, as_bytes(before)))

@@ -233,7 +233,10 @@ def test_experts_of_a_training_step():
     same step in 64 bits without sorting.  And the forward pass on the bf16 expert GEMM."""
     m, E, topk, hidden, ffn, cap = 90, 8, 2, 64, 48, 20
     gen = torch.Generator(device=DEV).manual_seed(3)
-    rand = lambda *s: torch.randn(s, generator=gen, device=DEV)
+
+    def rand(*s):
+        return torch.randn(s, generator=gen, device=DEV)
+
     idx = torch.rand(m, E, generator=gen, device=DEV).topk(topk, dim=1).indices
     x, logits, w = rand(m, hidden), rand(m, topk), rand(E, hidden, hidden) * hidden ** -0.5
     g = rand(m, hidden)
