@@ -326,11 +326,10 @@ __global__ void __launch_bounds__(kThreads) permute_kernel(const PermuteCall c) 
 
 // ------------------------------------------------------------------- unpermute ----
 
-// A warp per (token, piece of its columns).  A lane has eight vectors in flight: kCols columns of
-// kRows rows.  4095 tokens of 8 rows of 7168 bf16: 84 us, 6.3 TB/s.
-template <typename T, int kVec, int kRows>
+// A warp per (token, piece of its columns); a lane has kCols columns of kRows rows in flight.  4095
+// tokens of 8 rows of 7168 bf16: 81 us, 6.5 TB/s.
+template <typename T, int kVec, int kRows, int kCols>
 __global__ void __launch_bounds__(kThreads) unpermute_kernel(const UnpermuteCall c) {
-  constexpr int kCols = 8 / kRows;
   using V = Vec<T, kVec>;
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
@@ -797,15 +796,17 @@ void launch_unpermute_tokens(const UnpermuteCall& call, cudaStream_t stream) {
   const int vec = alignment(16, {address(c.y), address(c.out), c.hidden * size, c.out_stride * size});
   with_type(c.type, vec, [&](auto t, auto v) {
     using T = decltype(t);
-    auto run = [&](auto* kernel, int cols) {
-      const int64_t pieces = ceil_div<int64_t>(c.hidden / v.value, 32 * cols);
-      launch(kernel, c, ceil_div<int64_t>(c.rows.num_tokens * pieces, kWarps), stream);
+    auto pieces = [&](int cols) {
+      return static_cast<int64_t>(c.rows.num_tokens) * ceil_div(c.hidden / v.value, 32 * cols);
     };
-    // us for 2, 4 and 8 rows at a time: 4096 tokens of 4096 bf16, top-2 18.6 / 18.7 / 41.4, top-1 13.0 /
-    // 16.5 / 32.7, top-4 29.2 / 25.3 / 45.1; of 2048, top-6 21.8 / 20.7 / 24.9; 4095 of 7168, top-8 93.4 /
-    // 83.5 / 95.3; 16 of 2048, top-8 4.2 / 3.0 / 2.7.
-    if (c.rows.topk <= 2) run(unpermute_kernel<T, v.value, 2>, 4);
-    else run(unpermute_kernel<T, v.value, 4>, 2);
+    // Where every warp has one piece at most the rows of a token come in fewer turns, otherwise two rows
+    // and columns at a time keep most bytes in flight.  us for 4 x 1 and 2 x 2 (and 4 x 2, 8 x 1), bf16: 16
+    // tokens of 2048, top-8 2.3, 3.1; 128 of 7168, top-8 3.7, 4.0; 512 of 7168 9.1, 8.4; 4095 of 7168 81.4,
+    // 81.4 (84.2, 96.5); 4096 of 4096, top-2 23.2, 14.6 (19.1, 41.9); of 2048, top-6 21.2, 18.2 (20.7, 25.3).
+    if (pieces(1) <= static_cast<int64_t>(get_sm_count()) * 32)
+      launch(unpermute_kernel<T, v.value, 4, 1>, c, ceil_div<int64_t>(pieces(1), kWarps), stream);
+    else
+      launch(unpermute_kernel<T, v.value, 2, 2>, c, ceil_div<int64_t>(pieces(2), kWarps), stream);
   });
 }
 
