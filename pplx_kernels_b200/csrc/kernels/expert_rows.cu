@@ -704,10 +704,10 @@ uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 // Twice the blocks that fill every SM with 2048 threads; they loop over the rest.  (Once or four
 // times as many: 4096 x 28672 floats quantised in 103, 90, 90 us for once, twice, four times; copies of
 // 4096 tokens of 2048 25.0, 23.2, 24.5 us; the gradients of 4095 x 8 rows of 7168 170, 165, 164 us; their
-// sum 90, 91, 92 us.  Once for small blocks: 8168 rows of 2048 bf16, 64 threads each, 8.7 and 10.8 us.)
+// sum 90, 91, 92 us.  Once for the smallest blocks, whose launches show.)
 unsigned blocks_for(int64_t wanted, int threads) {
   const int64_t most = static_cast<int64_t>(get_sm_count()) * std::min(32, 2048 / threads) *
-                       (threads < 128 ? 1 : 2);
+                       (threads < 64 ? 1 : 2);
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(wanted, most)));
 }
 
@@ -859,10 +859,21 @@ void launch_quantize_rows(const QuantizeRowsCall& call, cudaStream_t stream) {
       if constexpr (v.value == 1) {
         run(quantize_ragged_kernel<T, kPermuted>, kThreads, items);
       } else {
+        // A warp per row up to 256 vectors, a block above; copies of many tokens, whose rounded values are
+        // stored several times, a block with eight vectors per thread above 128.  us for a block with four vectors per
+        // thread, a warp with eight, a block with eight: 8168 rows of 2048 bf16 8.3, 7.3, 8.4; of 1408 7.8,
+        // 6.8, 7.7; of 4096 15.9, -, 16.0; 4096 of 7168 14.7, -, 15.1; 4096 tokens of 2048 copied to 6 rows
+        // 12.5, 13.3, 11.8; 1021 of 7168 to 8 rows 14.0, -, 13.4; 77 of 7168 5.1, -, 7.2.
+        const int64_t by_warps = ceil_div<int64_t>(items, kWarps);
         if (vecs <= 32 * 4)
-          return run(quantize_kernel<T, v.value, 4, true, kPermuted>, kThreads, ceil_div<int64_t>(items, kWarps));
-        if (vecs <= kThreads * 4)
-          return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32), items);
+          return run(quantize_kernel<T, v.value, 4, true, kPermuted>, kThreads, by_warps);
+        if constexpr (!kPermuted) {
+          if (vecs <= 32 * 8)
+            return run(quantize_kernel<T, v.value, 8, true, kPermuted>, kThreads, by_warps);
+        }
+        if (vecs <= kThreads * 4 && (!kPermuted || items <= 4 * get_sm_count()))
+          return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32),
+                     items);
         const int threads = std::min(kThreads, round_up(ceil_div(vecs, 8), 32));
         run(quantize_kernel<T, v.value, 8, false, kPermuted>, threads, items);
       }
