@@ -871,7 +871,7 @@ void launch_quantize_rows(const QuantizeRowsCall& call, cudaStream_t stream) {
           if (vecs <= 32 * 8)
             return run(quantize_kernel<T, v.value, 8, true, kPermuted>, kThreads, by_warps);
         }
-        if (vecs <= kThreads * 4 && (!kPermuted || items <= 4 * get_sm_count()))
+        if (vecs <= kThreads * 4 && (!kPermuted || r.num_tokens <= 4 * get_sm_count()))
           return run(quantize_kernel<T, v.value, 4, false, kPermuted>, round_up(ceil_div(vecs, 4), 32),
                      items);
         const int threads = std::min(kThreads, round_up(ceil_div(vecs, 8), 32));
