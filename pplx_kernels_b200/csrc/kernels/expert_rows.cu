@@ -382,11 +382,13 @@ __global__ void __launch_bounds__(kThreads) unpermute_kernel(const UnpermuteCall
   }
 }
 
-// A block per token; behind the tokens, a block per row to be cleared.
+// A block per token; behind the tokens, a block per row to be cleared.  The gradient of a weight is a
+// sum over thousands of products that largely cancel: those of a vector are summed in 32 bits, the
+// vectors in 64.
 template <typename T, int kVec, int kRows, int kCols>
 __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const UnpermuteBackwardCall c) {
   using V = Vec<T, kVec>;
-  __shared__ float part[kRows][kWarps];
+  __shared__ double part[kRows][kWarps];
   const ExpertRowsView& r = c.rows;
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const Unpe
         my_row = row_at(r, t, k0 + lane);
         my_w = c.weights[t * r.topk + k0 + lane];
       }
-      float dot[kRows] = {};
+      double dot[kRows] = {};
       for (int first = 0; first < vecs; first += threads * kCols) {  // (the same for all threads)
         const int col0 = first + tid;
         V g[kCols], y[kRows][kCols];
@@ -456,24 +458,27 @@ __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const Unpe
 #pragma unroll
           for (int b = 0; b < kRows; ++b)
 #pragma unroll
-            for (int i = 0; i < kCols; ++i)
+            for (int i = 0; i < kCols; ++i) {
+              float sum = 0.0f;
 #pragma unroll
-              for (int j = 0; j < kVec; ++j) dot[b] = fmaf(y[b][i].get(j), g[i].get(j), dot[b]);
+              for (int j = 0; j < kVec; ++j) sum = fmaf(y[b][i].get(j), g[i].get(j), sum);
+              dot[b] += static_cast<double>(sum);
+            }
         }
       }
       if (c.grad_weights == nullptr) continue;
 #pragma unroll
       for (int b = 0; b < kRows; ++b) {
-        float s = dot[b];
+        double s = dot[b];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
         if (lane == 0) part[b][warp] = s;
       }
       __syncthreads();
       if (tid < kRows && k0 + tid < r.topk) {
-        float s = 0.0f;
+        double s = 0.0;
         for (int w2 = 0; w2 < threads / 32; ++w2) s += part[tid][w2];
-        c.grad_weights[t * r.topk + k0 + tid] = s;
+        c.grad_weights[t * r.topk + k0 + tid] = static_cast<float>(s);
       }
       __syncthreads();
     }
