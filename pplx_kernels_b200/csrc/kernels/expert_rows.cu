@@ -808,10 +808,13 @@ void launch_unpermute_tokens(const UnpermuteCall& call, cudaStream_t stream) {
     // and columns at a time keep most bytes in flight.  us for 4 x 1 and 2 x 2 (and 4 x 2, 8 x 1), bf16: 16
     // tokens of 2048, top-8 2.3, 3.1; 128 of 7168, top-8 3.7, 4.0; 512 of 7168 9.1, 8.4; 4095 of 7168 81.4,
     // 81.4 (84.2, 96.5); 4096 of 4096, top-2 23.2, 14.6 (19.1, 41.9); of 2048, top-6 21.2, 18.2 (20.7, 25.3).
+    // Rows of odd width, whose vectors are single values, take four columns: 4095 of 3971, top-8 141 us with
+    // two, 116 with four, 127 with eight; 300 of 1001, top-6 4.0, 3.8, 5.1.
+    constexpr int kCols = v.value * sizeof(T) == 2 ? 4 : 2;
     if (pieces(1) <= static_cast<int64_t>(get_sm_count()) * 32)
       launch(unpermute_kernel<T, v.value, 4, 1>, c, ceil_div<int64_t>(pieces(1), kWarps), stream);
     else
-      launch(unpermute_kernel<T, v.value, 2, 2>, c, ceil_div<int64_t>(pieces(2), kWarps), stream);
+      launch(unpermute_kernel<T, v.value, 2, kCols>, c, ceil_div<int64_t>(pieces(kCols), kWarps), stream);
   });
 }
 
@@ -825,8 +828,9 @@ void launch_unpermute_backward(const UnpermuteBackwardCall& c, cudaStream_t stre
     using T = decltype(t);
     // us for 2 rows x 2 columns, 2 x 4, 4 x 1, 8 x 1: 4096 tokens of 4096 bf16, top-2 28.3, 30.0, 34.1, 50.3;
     // top-4 50.8, 51.4, 50.2, 60.5; of 2048, top-6 38.2, 38.2, 42.9, 42.5; 4095 of 7168, top-8 159, 172,
-    // 161, 160; 16 of 2048, top-8 4.9, 5.0, 3.7, 3.4.
-    constexpr int kRows = 2, kCols = 2;
+    // 161, 160; 16 of 2048, top-8 4.9, 5.0, 3.7, 3.4.  Single values (odd widths) with four columns: 4095 of
+    // 3971, top-8 194 -> 175 us, 16 of 999 7.0 -> 6.0.
+    constexpr int kRows = 2, kCols = v.value * sizeof(T) == 2 ? 4 : 2;
     // As few threads as cover a token's vectors in whole turns of the block.
     const int vecs = c.hidden / v.value;
     const int turns = std::max(1, ceil_div(vecs, kThreads * kCols));
