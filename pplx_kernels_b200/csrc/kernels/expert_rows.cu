@@ -478,7 +478,9 @@ __global__ void __launch_bounds__(kThreads) unpermute_backward_kernel(const Unpe
       if (tid < kRows && k0 + tid < r.topk) {
         double s = 0.0;
         for (int w2 = 0; w2 < threads / 32; ++w2) s += part[tid][w2];
-        c.grad_weights[t * r.topk + k0 + tid] = static_cast<float>(s);
+        // (Without a row it is zero whatever the gradient is: zeros times infinity are not.  Lane tid of the
+        // first warp holds the row.)
+        c.grad_weights[t * r.topk + k0 + tid] = my_row >= 0 ? static_cast<float>(s) : 0.0f;
       }
       __syncthreads();
     }

@@ -295,6 +295,31 @@ def test_permute_int8(dtype, m, topk, hidden, capacity):
         assert (q2[~there] == fill).all() and (s2[~there] == fill).all()
 
 
+@pytest.mark.parametrize("hidden", [33, 256, 2048])
+def test_gradients_that_are_not_finite(hidden):
+    """An infinity or a NaN reaches its own token's entries, and of those only the ones with a row."""
+    m, topk, experts = 12, 5, 4
+    indices = routing(m, topk, experts)
+    indices[::2, 3] = -1
+    indices[4] = -1
+    rows = sort_by_expert(indices, experts)
+    y, w = data(m * topk, hidden), torch.rand(m, topk, device=DEV) + 0.5
+    g = data(m, hidden, seed=3)
+    want_y, want_w = unpermute_tokens_backward(g, y, rows, w)
+    bad = g.clone()
+    bad[2, 0], bad[4, hidden - 1], bad[6] = float("inf"), float("nan"), float("-inf")
+    grad_y, grad_w = unpermute_tokens_backward(bad, y, rows, w)
+    there = rows.row_of >= 0
+    hit = torch.zeros(m, 1, dtype=torch.bool, device=DEV)
+    hit[[2, 4, 6]] = True
+    assert torch.equal(grad_w[~(hit & there)], want_w[~(hit & there)])
+    assert (grad_w[~there] == 0).all() and not grad_w[hit & there].isfinite().any()
+    touched = torch.zeros(m * topk, dtype=torch.bool, device=DEV)
+    touched[rows.row_of[hit & there].long()] = True
+    assert torch.equal(grad_y[~touched], want_y[~touched])
+    assert not grad_y[touched].isfinite().all(1).any()
+
+
 def test_rows_out_of_range_are_skipped():
     """A table that does not fit the tensors: the kernels leave such entries out."""
     m, topk, hidden = 4, 2, 32
