@@ -621,11 +621,11 @@ __global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
 // thread and turn, read one by one and (after the search for the largest) from the caches.  A row of q
 // may begin at any byte: a thread stores the aligned word that its values and those of the lane below
 // make up, and the ends of the row one byte at a time.
-template <typename T, bool kPermuted>
-__global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const QuantizeRowsCall c,
-                                                                   const ExpertRowsView r) {
+template <typename T, bool kPermuted, int kBlock>
+__global__ void __launch_bounds__(kBlock) quantize_ragged_kernel(const QuantizeRowsCall c,
+                                                                 const ExpertRowsView r) {
   using V = Vec<T, 1>;
-  __shared__ uint32_t part[2][kWarps];
+  __shared__ uint32_t part[2][kBlock / 32];
   ptx::wait_for_previous_kernels();
   ptx::let_next_kernel_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const Quantiz
     if (t >= sources) {
       const int64_t row = rest_row(r, rest, t - sources);
       if (row < 0) continue;
-      for (int col = tid; col < c.hidden; col += kThreads) c.q[row * c.hidden + col] = 0;
+      for (int col = tid; col < c.hidden; col += kBlock) c.q[row * c.hidden + col] = 0;
       if (tid == 0) c.scale[row] = 0.0f;
       continue;
     }
@@ -652,13 +652,13 @@ __global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const Quantiz
       return v.get(0);
     };
     uint32_t bits = 0;
-    for (int col = tid; col < c.hidden; col += 4 * kThreads)
+    for (int col = tid; col < c.hidden; col += 4 * kBlock)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bits = max(bits, magnitude(value(col + i * kThreads)));
+      for (int i = 0; i < 4; ++i) bits = max(bits, magnitude(value(col + i * kBlock)));
     bits = __reduce_max_sync(kAll, bits);
     if (lane == 0) part[turn][warp] = bits;
     __syncthreads();
-    bits = __reduce_max_sync(kAll, lane < kWarps ? part[turn][lane] : 0u);
+    bits = __reduce_max_sync(kAll, lane < kBlock / 32 ? part[turn][lane] : 0u);
     turn ^= 1;  // (the next row's maxima go elsewhere, so one barrier is enough)
     const float amax = row_amax(bits);
     const float inv = 127.0f / amax, scale = amax / 127.0f;
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const Quantiz
     if (kPermuted && lane < r.topk) my_row = row_at(r, t, lane);
     // A warp makes 32 words and stores 31: the lowest lane only hands its values up.  (The last word of
     // a row that begins inside one is behind the row's last values.)
-    for (int turn_of = warp; turn_of * 31 * 4 < c.hidden + 4; turn_of += kWarps) {
+    for (int turn_of = warp; turn_of * 31 * 4 < c.hidden + 4; turn_of += kBlock / 32) {
       const int col = (turn_of * 31 + lane - 1) * 4;
       uint32_t word = 0;
       if (col >= 0) word = keep & quantize(value(col), value(col + 1), value(col + 2), value(col + 3), inv);
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kThreads) quantize_ragged_kernel(const Quantiz
         }
       }
     }
-    for (int k = tid; k < targets; k += kThreads) {
+    for (int k = tid; k < targets; k += kBlock) {
       const int64_t row = kPermuted ? row_at(r, t, k) : t;
       if (row >= 0) c.scale[row] = scale;
     }
@@ -868,7 +868,12 @@ void launch_quantize_rows(const QuantizeRowsCall& call, cudaStream_t stream) {
     auto pick = [&](auto permuted) {
       constexpr bool kPermuted = decltype(permuted)::value;
       if constexpr (v.value == 1) {
-        run(quantize_ragged_kernel<T, kPermuted>, kThreads, items);
+        // us with 256 and 64 threads: 30000 rows of 33 bf16 35.9, 16.4; 4095 of 401 7.2, 4.9; of 1001 9.5, 7.4;
+        // 8168 of 2047 23.0, 18.9; 4095 of 3971 18.4, 19.3; 200 of 7001 4.8, 10.5; 4095 tokens copied to 8
+        // rows, of 401 19.1, 11.9, of 1001 31.6, 24.0, of 3971 70.6, 78.4; 1 of 2047 6.6, 13.8.
+        if (c.hidden <= 512 || (c.hidden <= 2048 && items > 8 * get_sm_count()))
+          run(quantize_ragged_kernel<T, kPermuted, 64>, 64, items);
+        else run(quantize_ragged_kernel<T, kPermuted, kThreads>, kThreads, items);
       } else {
         // A warp per row up to 256 vectors, a block above; copies of many tokens, whose rounded values are
         // stored several times, a block with eight vectors per thread above 128.  us for a block with four vectors per
