@@ -280,10 +280,8 @@ def _spread(x: torch.Tensor, token: torch.Tensor) -> torch.Tensor:
 def _plain_quantize(x: torch.Tensor):
     v = x.float()
     amax = v.abs().amax(dim=-1).clamp(min=TINY)
-    # (A quotient of two tensors is one; with a number torch multiplies by a rounded reciprocal.)
-    most = torch.full_like(amax, 127.0)
-    q = torch.round(v * (most / amax).unsqueeze(-1)).clamp(-127, 127).to(torch.int8)
-    return q, amax / most
+    q = torch.round(v * (127.0 / amax).unsqueeze(-1)).clamp(-127, 127).to(torch.int8)
+    return q, amax / 127.0
 
 
 def _plain_gemm(s, xq, x_scale, w, w_scale, counts, offsets, padded, up, dtype):
