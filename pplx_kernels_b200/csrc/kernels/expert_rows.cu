@@ -499,6 +499,13 @@ __device__ __forceinline__ float row_amax(uint32_t bits) {
   return __uint_as_float(max(bits, __float_as_uint(1e-30f)));
 }
 
+// The row's factor by its rounded reciprocal and its scale by the rounded 1/127: products take the place
+// of quotients, as in torch's `127.0 / a` and `a / 127.0`.  Each is within 2 roundings of the quotient
+// (the reciprocal of a > 8.5e37 is subnormal: 2^-22 of it at most), and decides only values that lie next to
+// the border of two integers.
+__device__ __forceinline__ float row_factor(float amax) { return __fmul_rn(127.0f, __frcp_rn(amax)); }
+__device__ __forceinline__ float row_scale(float amax) { return __fmul_rn(amax, 1.0f / 127.0f); }
+
 // rint(v * inv) of four values, |v * inv| <= 127.0001, as bytes: adding 1.5 * 2^23 rounds to whole
 // numbers, which are then the low bits.  (The product is rounded before: no fused add.)
 __device__ __forceinline__ uint32_t quantize(float a, float b, float c, float d, float inv) {
@@ -571,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 4 ? 6 : 3)
       turn ^= 1;  // (the next row's maxima go elsewhere, so one barrier is enough)
     }
     const float amax = row_amax(bits);
-    const float inv = 127.0f / amax, scale = amax / 127.0f;
+    const float inv = row_factor(amax), scale = row_scale(amax);
     // A row with an infinity or a NaN is zero throughout.
     const uint32_t keep = amax < __uint_as_float(0x7f800000u) ? 0xffffffffu : 0u;
     auto rounded = [&](const V& v) {
@@ -661,7 +668,7 @@ __global__ void __launch_bounds__(kBlock) quantize_ragged_kernel(const QuantizeR
     bits = __reduce_max_sync(kAll, lane < kBlock / 32 ? part[turn][lane] : 0u);
     turn ^= 1;  // (the next row's maxima go elsewhere, so one barrier is enough)
     const float amax = row_amax(bits);
-    const float inv = 127.0f / amax, scale = amax / 127.0f;
+    const float inv = row_factor(amax), scale = row_scale(amax);
     const uint32_t keep = amax < __uint_as_float(0x7f800000u) ? 0xffffffffu : 0u;
     const int targets = kPermuted ? r.topk : 1;
     int my_row = -1;  // lane k holds that of entry k

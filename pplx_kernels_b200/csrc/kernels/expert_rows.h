@@ -78,7 +78,8 @@ struct UnpermuteBackwardCall {
 };
 void launch_unpermute_backward(const UnpermuteBackwardCall& call, cudaStream_t stream);
 
-// Rows to 8-bit integers: scale = max(max |x|, 1e-30) / 127, q = rint(x * (127 / max(...))).
+// Rows to 8-bit integers: a = max(max |x|, 1e-30), scale = a * (1 / 127), q = rint(x * (127 * (1 / a))), each
+// step rounded to fp32.
 // `rows` given: the row of token t goes to every row_of[t, k] (zero_rest as above).  Otherwise row
 // r of `num_rows` goes to row r; with `counts`, rows r % plane_rows >= counts[r / plane_rows] are
 // skipped.

@@ -48,11 +48,12 @@ def quantize_rows_int8(x: torch.Tensor, counts: torch.Tensor | None = None,
     """Rows of 8-bit integers with one fp32 scale each: ``x ~= q * scale``.
 
     ``x`` [rows, k] or [experts, rows, k] in bf16, fp16 or fp32 (weights, one row per channel, or
-    activations).  With ``a = max(max |x|, 1e-30)`` of a row, ``scale = a / 127`` and ``q =
-    round(x * (127 / a))``, ties to even, in fp32, within [-127, 127].  A row with an
-    infinity or a NaN gets that as its scale and zeros in place of the value, so that what is
-    computed with the row is not finite either.  ``counts`` [experts] int32, with x of [experts,
-    rows, k]: rows at or beyond an expert's count are left as they are.
+    activations).  With ``a = max(max |x|, 1e-30)`` of a row, ``scale = a * (1 / 127)`` and ``q =
+    round(x * (127 * (1 / a)))``, ties to even, within [-127, 127]; each step is rounded to fp32, the
+    reciprocals too, so a value on the border of two integers goes where its rounded product lies.
+    A row with an infinity or a NaN gets that as its scale and zeros in place of the values, so
+    that what is computed with the row is not finite either.  ``counts`` [experts] int32, with x of
+    [experts, rows, k]: rows at or beyond an expert's count are left as they are.
     """
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("quantize_rows_int8: no gradient is recorded here; use torch.no_grad() or detach()")
@@ -70,7 +71,6 @@ def quantize_rows_int8_reference(x: torch.Tensor) -> tuple[torch.Tensor, torch.T
     """Plain PyTorch statement of ``quantize_rows_int8`` for finite rows."""
     v = x.to(torch.float32)
     amax = v.abs().amax(dim=-1).clamp(min=1e-30)
-    # (A quotient of two tensors is one; with a number torch multiplies by a rounded reciprocal.)
-    most = torch.full_like(amax, 127.0)
-    q = torch.round(v * (most / amax).unsqueeze(-1)).clamp(-127, 127).to(torch.int8)
-    return q, amax / most
+    q = torch.round(v * (127.0 * amax.reciprocal()).unsqueeze(-1)).clamp(-127, 127).to(torch.int8)
+    # (As a tensor, so that the reciprocal is rounded to fp32 on every device.)
+    return q, amax * torch.full_like(amax, 127.0).reciprocal()
