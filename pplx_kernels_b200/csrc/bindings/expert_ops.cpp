@@ -415,9 +415,31 @@ class Sum : public torch::autograd::Function<Sum> {  // unpermute without weight
   }
 };
 
+// No operator has a forward-mode derivative: a tangent would be dropped without a word and count as
+// zero in what follows, so a tensor that carries one is refused.
+void check_no_tangent(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": ", name,
+              " carries a tangent; forward-mode derivatives are not implemented");
+}
+
+// What operators without a gradient of their own do in place of recording one.
+void not_differentiable(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
+                        torch::jit::Stack* stack) {
+  const c10::FunctionSchema& schema = op.schema();
+  const char* name = schema.name().c_str() + schema.name().rfind(':') + 1;
+  const size_t n = schema.arguments().size(), first = stack->size() - n;
+  for (size_t i = 0; i < n; ++i) {
+    const c10::IValue& v = (*stack)[first + i];
+    if (!v.isTensor() || !v.toTensor().defined()) continue;
+    check_no_tangent(v.toTensor(), name, schema.arguments()[i].name().c_str());
+  }
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+}
+
 at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts,
                                    const at::Tensor& offsets, const at::Tensor& row_of,
                                    int64_t capacity, bool zero_rest) {
+  check_no_tangent(x, "permute_tokens", "x");
   if (at::GradMode::is_enabled() && x.requires_grad())
     return Permute::apply(x, counts, offsets, row_of, capacity);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -427,6 +449,8 @@ at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts
 at::Tensor unpermute_tokens_autograd(const at::Tensor& y, const at::Tensor& counts,
                                      const at::Tensor& offsets, const at::Tensor& row_of,
                                      int64_t capacity, const std::optional<at::Tensor>& weights) {
+  check_no_tangent(y, "unpermute_tokens", "y");
+  if (weights.has_value()) check_no_tangent(*weights, "unpermute_tokens", "weights");
   if (at::GradMode::is_enabled()) {
     if (weights.has_value() && (y.requires_grad() || weights->requires_grad()))
       return Unpermute::apply(y, *weights, counts, offsets, row_of, capacity);
@@ -630,6 +654,11 @@ void register_expert_ops(torch::Library& m) {
         "Tensor? offsets, Tensor! out, bool swiglu, Tensor!? status, int expected_rows=0) -> ()");
   m.impl("grouped_gemm_int8", c10::kCUDA, &grouped_gemm_int8_op);
   m.impl("grouped_gemm_int8", c10::kMeta, &grouped_gemm_int8_op);
+  for (const char* op : {"permute_tokens_out", "permute_tokens_int8", "permute_tokens_int8_out",
+                         "unpermute_tokens_out", "unpermute_tokens_backward", "quantize_rows_int8",
+                         "quantize_rows_int8_out", "grouped_gemm_int8"})
+    m.impl(op, c10::DispatchKey::Autograd,
+           torch::CppFunction::makeFromBoxedFunction<&not_differentiable>());
 }
 
 }  // namespace pplx

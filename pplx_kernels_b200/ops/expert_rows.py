@@ -9,7 +9,8 @@ experts of an expert-parallel rank after its own exchange), the tokens need no a
     out = unpermute_tokens(y_rows, rows, weights)        # the weighted sum of each token's rows
 
 ``permute_tokens`` and ``unpermute_tokens`` are differentiable in the tokens, the rows and the
-weights.  ``permute_tokens_int8`` quantises on the way, for ``grouped_gemm_int8``.  The reference
+weights, in reverse mode; tensors that carry a forward-mode tangent are refused here and by the
+quantisation and the product of 8-bit integers.  ``permute_tokens_int8`` quantises on the way, for ``grouped_gemm_int8``.  The reference
 library has no such operators: its tokens always pass through dispatch and combine.
 
 Two layouts of the rows.  ``capacity=0``: one expert's rows after the other's, as many as there are

@@ -1,0 +1,80 @@
+"""What autograd meets in the operators of the experts of one GPU, on Meta tensors."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from pplx_kernels_b200.ops.expert_rows import (
+    permute_tokens,
+    permute_tokens_backward,
+    permute_tokens_int8,
+    sort_by_expert,
+    unpermute_tokens,
+    unpermute_tokens_backward,
+)
+from pplx_kernels_b200.ops.grouped_gemm import grouped_gemm_int8
+from pplx_kernels_b200.ops.quant import quantize_rows_int8
+
+M, K, E, H = 6, 3, 5, 64
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def rows():
+    return sort_by_expert(meta(M, K, dtype=torch.int32), E)
+
+
+def product(x_scale, w_scale, **kwargs):
+    return grouped_gemm_int8(meta(E, 4, H, dtype=torch.int8), x_scale, meta(E, 16, H, dtype=torch.int8),
+                             w_scale, **kwargs)
+
+
+# A call in one floating tensor, and its shape.
+FLOATING = {
+    "copy": (lambda t: permute_tokens(t, rows()), (M, H)),
+    "copy, out": (lambda t: permute_tokens(t, rows(), out=meta(M * K, H)), (M, H)),
+    "copy, into": (lambda t: permute_tokens(meta(M, H), rows(), out=t), (M * K, H)),
+    "copy, gradient": (lambda t: permute_tokens_backward(t, rows()), (M * K, H)),
+    "quantising copy": (lambda t: permute_tokens_int8(t, rows()), (M, H)),
+    "quantising copy, out": (lambda t: permute_tokens_int8(t, rows(), out=meta(M * K, H, dtype=torch.int8)),
+                             (M, H)),
+    "quantising copy, scale": (lambda t: permute_tokens_int8(meta(M, H), rows(), out_scale=t), (M * K,)),
+    "sum": (lambda t: unpermute_tokens(t, rows()), (M * K, H)),
+    "sum, weighted": (lambda t: unpermute_tokens(t, rows(), meta(M, K)), (M * K, H)),
+    "sum, weights": (lambda t: unpermute_tokens(meta(M * K, H), rows(), t), (M, K)),
+    "sum, out": (lambda t: unpermute_tokens(t, rows(), out=meta(M, H)), (M * K, H)),
+    "sum, weights, out": (lambda t: unpermute_tokens(meta(M * K, H), rows(), t, out=meta(M, H)), (M, K)),
+    "sum, gradient": (lambda t: unpermute_tokens_backward(t, meta(M * K, H), rows(), meta(M, K)), (M, H)),
+    "sum, gradient, rows": (lambda t: unpermute_tokens_backward(meta(M, H), t, rows(), meta(M, K)),
+                            (M * K, H)),
+    "quantisation": (lambda t: quantize_rows_int8(t), (M, H)),
+    "quantisation, out": (lambda t: quantize_rows_int8(t, out=meta(M, H, dtype=torch.int8)), (M, H)),
+    "product, scales": (lambda t: product(t, meta(E, 16)), (E, 4)),
+    "product, weights' scales": (lambda t: product(meta(E, 4), t), (E, 16)),
+}
+
+
+@pytest.mark.parametrize("name", FLOATING)
+@pytest.mark.parametrize("recorded", [False, True])
+def test_tangents_are_refused(name, recorded):
+    call, shape = FLOATING[name]
+    t = meta(*shape)
+    call(t)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t.requires_grad_(recorded), meta(*shape))
+        with pytest.raises((RuntimeError, ValueError), match="tangent|gradient"):
+            call(dual)
+    if not recorded:
+        with pytest.raises(RuntimeError, match="tangent"):
+            torch.func.jvp(call, (t,), (meta(*shape),))
+
+
+def test_tangents_through_a_gradient_are_refused():
+    """Forward over reverse: the gradient's own tangent."""
+    y, w, g = meta(M * K, H).requires_grad_(), meta(M, K).requires_grad_(), meta(M, H)
+    out = unpermute_tokens(y, rows(), w)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            torch.autograd.grad(out, (y, w), forward_ad.make_dual(g, meta(M, H)))
