@@ -422,18 +422,29 @@ void check_no_tangent(const at::Tensor& t, const char* op, const char* name) {
               " carries a tangent; forward-mode derivatives are not implemented");
 }
 
-// What operators without a gradient of their own do in place of recording one.
+// What operators without a gradient of their own do in place of recording one.  A tensor that is written
+// counts as changed, so that a backward pass that saved it notices; one that a gradient is recorded for
+// is refused, as by torch's own `out=`.
 void not_differentiable(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
                         torch::jit::Stack* stack) {
   const c10::FunctionSchema& schema = op.schema();
   const char* name = schema.name().c_str() + schema.name().rfind(':') + 1;
+  c10::SmallVector<at::Tensor, 4> written;
   const size_t n = schema.arguments().size(), first = stack->size() - n;
   for (size_t i = 0; i < n; ++i) {
     const c10::IValue& v = (*stack)[first + i];
     if (!v.isTensor() || !v.toTensor().defined()) continue;
-    check_no_tangent(v.toTensor(), name, schema.arguments()[i].name().c_str());
+    const at::Tensor& t = v.toTensor();
+    const c10::Argument& argument = schema.arguments()[i];
+    check_no_tangent(t, name, argument.name().c_str());
+    if (argument.alias_info() == nullptr || !argument.alias_info()->isWrite()) continue;
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, ": ", argument.name(),
+                " is written and requires a gradient, which is not recorded; use torch.no_grad() or detach()");
+    written.push_back(t);
   }
   op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+  for (const at::Tensor& t : written)
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
 }
 
 at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts,

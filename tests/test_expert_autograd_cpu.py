@@ -78,3 +78,64 @@ def test_tangents_through_a_gradient_are_refused():
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="tangent"):
             torch.autograd.grad(out, (y, w), forward_ad.make_dual(g, meta(M, H)))
+
+
+# Calls that write tensors: what they write.
+WRITING = {
+    "copy": lambda o: permute_tokens(meta(M, H), rows(), out=o[0]),
+    "quantising copy": lambda o: permute_tokens_int8(meta(M, H), rows(), out=o[1], out_scale=o[2]),
+    "sum": lambda o: unpermute_tokens(meta(M * K, H), rows(), out=o[0][:M]),
+    "quantisation": lambda o: quantize_rows_int8(meta(M * K, H), out=o[1], out_scale=o[2]),
+    "product": lambda o: product(meta(E, 4), meta(E, 16), out=o[3], status=o[4]),
+}
+
+
+def buffers():
+    return [meta(M * K, H), meta(M * K, H, dtype=torch.int8), meta(M * K),
+            meta(E, 4, 16, dtype=torch.bfloat16), meta(1, dtype=torch.int32)]
+
+
+@pytest.mark.parametrize("name", WRITING)
+def test_written_tensors_count_as_changed(name):
+    written = {"copy": [0], "sum": [0], "product": [3, 4]}.get(name, [1, 2])
+    o = buffers()
+    WRITING[name](o)
+    assert [t._version for t in o] == [int(i in written) for i in range(5)]
+    with torch.no_grad():
+        WRITING[name](o)
+    assert [t._version for t in o] == [2 * int(i in written) for i in range(5)]
+    with torch.inference_mode():
+        WRITING[name](buffers())  # (tensors without a version)
+    inference = buffers()
+    with torch.inference_mode():
+        inference = buffers()
+    WRITING[name](inference)
+
+
+def test_a_saved_tensor_that_is_overwritten_is_noticed():
+    x, out = meta(M * K, H).requires_grad_(), meta(M * K, H)
+    y = (x * out).sum()
+    permute_tokens(meta(M, H), rows(), out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("name", WRITING)
+def test_written_tensors_that_require_a_gradient_are_refused(name):
+    o = buffers()
+    for t in o:
+        if t.is_floating_point():
+            t.requires_grad_()
+    with torch.no_grad():
+        WRITING[name](o)
+    with pytest.raises((RuntimeError, ValueError), match="gradient"):
+        WRITING[name](o)
+
+
+def test_gradients_leave_the_saved_tensors_alone():
+    """The backward pass writes its results only."""
+    y, w = meta(M * K, H).requires_grad_(), meta(M, K).requires_grad_()
+    where = rows()
+    unpermute_tokens(y, where, w).sum().backward()
+    unpermute_tokens_backward(meta(M, H), y.detach(), where, w.detach())
+    assert y._version == w._version == where.row_of._version == 0
