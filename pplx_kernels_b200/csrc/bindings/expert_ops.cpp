@@ -283,7 +283,7 @@ at::Tensor unpermute_tokens_op(const at::Tensor& y, const at::Tensor& counts,
   return out;
 }
 
-void unpermute_tokens_backward_op(const at::Tensor& grad, const at::Tensor& y,
+void unpermute_tokens_backward_op(const at::Tensor& grad, const std::optional<at::Tensor>& y,
                                   const at::Tensor& counts, const at::Tensor& offsets,
                                   const at::Tensor& row_of, int64_t capacity,
                                   const at::Tensor& weights,
@@ -298,15 +298,18 @@ void unpermute_tokens_backward_op(const at::Tensor& grad, const at::Tensor& y,
   const int64_t hidden = grad.size(1);
   check_hidden(hidden, op);
   TORCH_CHECK(grad.size(0) == c.rows.num_tokens, op, ": grad and row_of disagree on the token count");
-  check_rows(y, c.rows, hidden, grad, op, "y");
-  TORCH_CHECK(y.scalar_type() == grad.scalar_type(), op, ": grad must have the type of y");
+  if (y.has_value()) {
+    check_rows(*y, c.rows, hidden, grad, op, "y");
+    TORCH_CHECK(y->scalar_type() == grad.scalar_type(), op, ": grad must have the type of y");
+    c.y = data<void>(*y);
+  }
+  TORCH_CHECK(y.has_value() || !grad_weights.has_value(), op, ": grad_weights needs y");
   c.weights = weights_ptr(weights, c.rows, grad, op);
   c.grad = data<void>(grad);
-  c.y = data<void>(y);
   c.hidden = static_cast<int>(hidden);
   if (grad_y.has_value()) {
     check_rows(*grad_y, c.rows, hidden, grad, op, "grad_y");
-    TORCH_CHECK(grad_y->scalar_type() == y.scalar_type(), op, ": grad_y must have the type of y");
+    TORCH_CHECK(grad_y->scalar_type() == grad.scalar_type(), op, ": grad_y must have the type of grad");
     c.grad_y = data<void>(*grad_y);
   }
   if (grad_weights.has_value()) {
@@ -341,9 +344,10 @@ at::Tensor call_unpermute(const at::Tensor& y, const at::Tensor& counts, const a
   return op.call(y, counts, offsets, row_of, capacity, weights);
 }
 
-void call_unpermute_backward(const at::Tensor& grad, const at::Tensor& y, const at::Tensor& counts,
-                             const at::Tensor& offsets, const at::Tensor& row_of, int64_t capacity,
-                             const at::Tensor& weights, const std::optional<at::Tensor>& grad_y,
+void call_unpermute_backward(const at::Tensor& grad, const std::optional<at::Tensor>& y,
+                             const at::Tensor& counts, const at::Tensor& offsets,
+                             const at::Tensor& row_of, int64_t capacity, const at::Tensor& weights,
+                             const std::optional<at::Tensor>& grad_y,
                              const std::optional<at::Tensor>& grad_weights) {
   static auto op = c10::Dispatcher::singleton()
                        .findSchemaOrThrow("pplx_kernels_b200::unpermute_tokens_backward", "")
@@ -376,24 +380,26 @@ class Unpermute : public torch::autograd::Function<Unpermute> {
                             const at::Tensor& counts, const at::Tensor& offsets,
                             const at::Tensor& row_of, int64_t capacity) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({y, weights, counts, offsets, row_of});
+    // (Only the gradient of the weights reads the rows: without it they need not be kept.)
+    ctx->save_for_backward({weights.requires_grad() ? y : at::Tensor(), weights, counts, offsets, row_of});
     ctx->saved_data["capacity"] = capacity;
     return call_unpermute(y, counts, offsets, row_of, capacity, weights);
   }
   static Variables backward(AutogradContext* ctx, const Variables& grads) {
     const Variables saved = ctx->get_saved_variables();
-    const at::Tensor &y = saved[0], &weights = saved[1];
+    const at::Tensor &y = saved[0], &weights = saved[1], grad = grads[0].contiguous();
+    const int64_t capacity = ctx->saved_data["capacity"].toInt();
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "unpermute_tokens: its gradient has no derivative of its own (create_graph)");
     at::Tensor grad_y, grad_weights;
-    if (ctx->needs_input_grad(0)) grad_y = at::empty_like(y);
+    if (ctx->needs_input_grad(0))
+      grad_y = empty_rows(grad, saved[2], saved[4], capacity, grad.scalar_type());
     if (ctx->needs_input_grad(1)) grad_weights = at::empty_like(weights);
     auto given = [](const at::Tensor& t) {
       return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
     };
-    call_unpermute_backward(grads[0].contiguous(), y, saved[2], saved[3], saved[4],
-                            ctx->saved_data["capacity"].toInt(), weights, given(grad_y),
-                            given(grad_weights));
+    call_unpermute_backward(grad, given(y), saved[2], saved[3], saved[4], capacity, weights,
+                            given(grad_y), given(grad_weights));
     return {grad_y, grad_weights, {}, {}, {}, {}};
   }
 };
@@ -651,7 +657,7 @@ void register_expert_ops(torch::Library& m) {
         "Tensor? weights, Tensor! out, Tensor? bound_m) -> ()");
   m.impl("unpermute_tokens_out", c10::kCUDA, &unpermute_tokens_out_op);
   m.impl("unpermute_tokens_out", c10::kMeta, &unpermute_tokens_out_op);
-  m.def("unpermute_tokens_backward(Tensor grad, Tensor y, Tensor counts, Tensor offsets, "
+  m.def("unpermute_tokens_backward(Tensor grad, Tensor? y, Tensor counts, Tensor offsets, "
         "Tensor row_of, int capacity, Tensor weights, Tensor!? grad_y, Tensor!? grad_weights) -> ()");
   m.impl("unpermute_tokens_backward", c10::kCUDA, &unpermute_tokens_backward_op);
   m.impl("unpermute_tokens_backward", c10::kMeta, &unpermute_tokens_backward_op);

@@ -70,7 +70,7 @@ struct UnpermuteBackwardCall {
   FloatType type = FloatType::kBFloat16;
   const void* grad = nullptr;
   int64_t grad_stride = 0;             // elements
-  const void* y = nullptr;
+  const void* y = nullptr;             // read for grad_weights only
   const float* weights = nullptr;
   void* grad_y = nullptr;              // optional
   float* grad_weights = nullptr;       // optional

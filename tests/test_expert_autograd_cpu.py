@@ -139,3 +139,26 @@ def test_gradients_leave_the_saved_tensors_alone():
     unpermute_tokens(y, where, w).sum().backward()
     unpermute_tokens_backward(meta(M, H), y.detach(), where, w.detach())
     assert y._version == w._version == where.row_of._version == 0
+
+
+@pytest.mark.parametrize("capacity", [0, 4])
+@pytest.mark.parametrize("of_rows,of_weights", [(True, True), (True, False), (False, True)])
+def test_rows_are_kept_for_the_gradient_of_the_weights_only(capacity, of_rows, of_weights):
+    """A frozen router: the gradient of the rows needs the weights and the grad, not the rows."""
+    where = sort_by_expert(meta(M, K, dtype=torch.int32), E, capacity)
+    y, w = meta(*where.shape(), H).requires_grad_(of_rows), meta(M, K).requires_grad_(of_weights)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.shape) or t, lambda t: t):
+        out = unpermute_tokens(y, where, w)
+    assert (y.shape in kept) == of_weights
+    out.sum().backward()
+    assert (y.grad is not None) == of_rows and (w.grad is not None) == of_weights
+    assert not of_rows or y.grad.shape == y.shape
+    assert not of_weights or w.grad.shape == w.shape
+
+
+def test_gradient_of_the_weights_without_rows_is_refused():
+    where = rows()
+    with pytest.raises(RuntimeError, match="needs y"):
+        torch.ops.pplx_kernels_b200.unpermute_tokens_backward(
+            meta(M, H), None, where.counts, where.offsets, where.row_of, 0, meta(M, K), None, meta(M, K))
