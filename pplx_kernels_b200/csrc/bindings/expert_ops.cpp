@@ -457,8 +457,11 @@ at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts
                                    const at::Tensor& offsets, const at::Tensor& row_of,
                                    int64_t capacity, bool zero_rest) {
   check_no_tangent(x, "permute_tokens", "x");
-  if (at::GradMode::is_enabled() && x.requires_grad())
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    // (Any type is copied, but the gradient is a sum of rows: refused here, not in the backward pass.)
+    float_type(x, "permute_tokens", "x, which requires a gradient,");
     return Permute::apply(x, counts, offsets, row_of, capacity);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   return call_permute(x, counts, offsets, row_of, capacity, zero_rest);
 }

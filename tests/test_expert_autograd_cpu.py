@@ -162,3 +162,14 @@ def test_gradient_of_the_weights_without_rows_is_refused():
     with pytest.raises(RuntimeError, match="needs y"):
         torch.ops.pplx_kernels_b200.unpermute_tokens_backward(
             meta(M, H), None, where.counts, where.offsets, where.row_of, 0, meta(M, K), None, meta(M, K))
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.complex64, torch.float8_e4m3fn])
+def test_types_without_a_gradient_are_refused_at_once(dtype):
+    x = meta(M, H, dtype=dtype)
+    assert permute_tokens(x, rows()).dtype == dtype
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="bfloat16, float16 or float32"):
+        permute_tokens(x, rows())
+    with torch.no_grad():
+        assert permute_tokens(x, rows()).dtype == dtype
