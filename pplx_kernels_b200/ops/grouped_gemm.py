@@ -150,8 +150,10 @@ def grouped_gemm_int8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
     result is ``silu(gate) * up``.  ``out`` is bf16 or fp16 (``out_dtype`` where it is allocated
     here), rounded once.  Rows without a token are left untouched.  ``status`` (int32, optional) is
     set to 1 if a wait ran out.  ``expected_rows`` (total valid rows, 0 = capacity) is a hint for
-    the choice of the kernel form.
+    the choice of the kernel form.  Not differentiable: scales that require a gradient are refused.
     """
+    if (x_scale.requires_grad or w_scale.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("grouped_gemm_int8: no gradient is recorded here; use torch.no_grad() or detach()")
     n_out = wq.size(1) // 2 if swiglu else wq.size(1)
     if out is None:
         out = torch.empty(*xq.shape[:-1], n_out, dtype=out_dtype, device=xq.device)

@@ -173,3 +173,12 @@ def test_types_without_a_gradient_are_refused_at_once(dtype):
         permute_tokens(x, rows())
     with torch.no_grad():
         assert permute_tokens(x, rows()).dtype == dtype
+
+
+def test_scales_of_a_product_that_require_a_gradient_are_refused():
+    for of_rows in (True, False):
+        scales = meta(E, 4).requires_grad_(of_rows), meta(E, 16).requires_grad_(not of_rows)
+        with pytest.raises(ValueError, match="gradient"):
+            product(*scales)
+        with torch.no_grad():
+            assert product(*scales).shape == (E, 4, 16)
