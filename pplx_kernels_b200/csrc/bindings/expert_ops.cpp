@@ -611,6 +611,10 @@ void grouped_gemm_int8_op(const at::Tensor& xq, const at::Tensor& x_scale, const
   c.out_stride_e = one_plane ? 0 : used_stride(out, 0, rows * c.out_stride_row);
   TORCH_CHECK(c.x_stride_row >= k && c.w_stride_row >= k && c.out_stride_row >= n_out, op,
               ": rows must not overlap");
+  // (Planes behind each other, or rows of all experts in turn.)
+  TORCH_CHECK(one_plane || E <= 1 || c.out_stride_e >= (rows - 1) * c.out_stride_row + n_out ||
+                  (c.out_stride_e >= n_out && c.out_stride_row >= (E - 1) * c.out_stride_e + n_out),
+              op, ": the experts' rows of out must not overlap");
   c.num_experts = static_cast<int>(E);
   c.rows_per_expert = static_cast<int>(rows);
   c.n_out = static_cast<int>(n_out);
