@@ -1,6 +1,7 @@
 // Operators of the experts of one GPU: tokens sorted by expert and back, with gradients, rows
 // quantised to 8-bit integers, and their grouped GEMM.  No counterpart in the reference.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -58,6 +59,15 @@ FloatType float_type(const at::Tensor& t, const char* op, const char* name) {
     case at::kFloat: return FloatType::kFloat;
     default: TORCH_CHECK(false, op, ": ", name, " must be bfloat16, float16 or float32");
   }
+}
+
+// Tokens and rows are read in an order of their own: a result in the memory of the input would be read
+// back as input.
+void check_apart(const at::Tensor& written, const at::Tensor& read, const char* op, const char* name,
+                 const char* from) {
+  const at::MemOverlapStatus s = at::get_overlap_status(written, read);
+  TORCH_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, op, ": ", name,
+              " must not share memory with ", from);
 }
 
 // [tokens, hidden] with contiguous columns; the distance of two rows in elements.
@@ -200,6 +210,7 @@ void permute_tokens_out_op(const at::Tensor& x, const at::Tensor& counts, const 
   check_hidden(x.size(1), op);
   check_rows(out, c.rows, x.size(1), x, op, "out");
   TORCH_CHECK(out.scalar_type() == x.scalar_type(), op, ": out must have the type of x");
+  check_apart(out, x, op, "out", "x");
   c.x = data<void>(x);
   c.out = data<void>(out);
   c.row_bytes = x.size(1) * x.element_size();
@@ -232,6 +243,8 @@ void permute_tokens_int8_out_op(const at::Tensor& x, const at::Tensor& counts, c
   TORCH_CHECK(out_scale.scalar_type() == at::kFloat && out_scale.is_contiguous() &&
                   out_scale.sizes() == out.sizes().slice(0, out.dim() - 1),
               op, ": out_scale must be contiguous float32, one per row of out");
+  check_apart(out, x, op, "out", "x");
+  check_apart(out_scale, x, op, "out_scale", "x");
   c.zero_rest = zero_rest;
   c.x = data<void>(x);
   c.q = data<int8_t>(out);
@@ -266,6 +279,7 @@ void unpermute_tokens_out_op(const at::Tensor& y, const at::Tensor& counts, cons
   TORCH_CHECK(out.size(0) >= c.rows.num_tokens, op, ": out has fewer rows than row_of");
   check_hidden(out.size(1), op);
   check_rows(y, c.rows, out.size(1), y, op, "y");
+  check_apart(out, y, op, "out", "y");
   if (weights.has_value()) c.weights = weights_ptr(*weights, c.rows, y, op);
   c.bound_m = bound_ptr(bound_m, y, op);
   c.y = data<void>(y);
@@ -504,6 +518,8 @@ void quantize_rows_int8_out_op(const at::Tensor& x, const std::optional<at::Tens
   TORCH_CHECK(out_scale.scalar_type() == at::kFloat && out_scale.is_contiguous() &&
                   out_scale.sizes() == x.sizes().slice(0, x.dim() - 1),
               op, ": out_scale must be contiguous float32, one per row of x");
+  check_apart(out, x, op, "out", "x");
+  check_apart(out_scale, x, op, "out_scale", "x");
   if (counts.has_value()) {
     check_device(*counts, x, op, "counts");
     TORCH_CHECK(x.dim() == 3 && counts->scalar_type() == at::kInt && counts->is_contiguous() &&
@@ -615,6 +631,7 @@ void grouped_gemm_int8_op(const at::Tensor& xq, const at::Tensor& x_scale, const
   TORCH_CHECK(one_plane || E <= 1 || c.out_stride_e >= (rows - 1) * c.out_stride_row + n_out ||
                   (c.out_stride_e >= n_out && c.out_stride_row >= (E - 1) * c.out_stride_e + n_out),
               op, ": the experts' rows of out must not overlap");
+  check_apart(out, xq, op, "out", "xq");
   c.num_experts = static_cast<int>(E);
   c.rows_per_expert = static_cast<int>(rows);
   c.n_out = static_cast<int>(n_out);
