@@ -773,9 +773,11 @@ void launch_sort_by_expert(const SortByExpertCall& c, cudaStream_t stream) {
   const int threads = n <= 256 ? 256 : kSortThreads;
   const int warps = threads / 32;
   const size_t smem = sizeof(uint32_t) * (static_cast<size_t>(warps + 3) * c.num_experts + 1);
+  // (The most that any call takes, not this one's: threads that launch with other sizes set it too.)
   if (smem > 48 * 1024)
-    CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(smem)));
+    CUDA_CHECK(cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        static_cast<int>(sizeof(uint32_t)) * ((kSortThreads / 32 + 3) * kMaxSortExperts + 1)));
   if (blocks > 8)
     CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   void* params[] = {const_cast<SortByExpertCall*>(&c)};

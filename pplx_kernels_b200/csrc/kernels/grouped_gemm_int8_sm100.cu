@@ -646,8 +646,9 @@ void launch_one(const CUtensorMap& tmap_w, const TokenMaps& tmap_x, Int8GemmArgs
                 "too little shared memory for the stages");
   g.ring_bytes = static_cast<uint32_t>((kSmem - fixed) & ~static_cast<size_t>(1023));
   const size_t smem = fixed + g.ring_bytes;
+  // (The most that any call takes, not this one's: threads that launch with other sizes set it too.)
   CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(smem)));
+                                  static_cast<int>(kSmem)));
   void* params[] = {const_cast<CUtensorMap*>(&tmap_w), const_cast<TokenMaps*>(&tmap_x), &g};
   CUDA_CHECK(launch_after_previous(reinterpret_cast<const void*>(kernel), dim3(kPair ? (grid & ~1) : grid),
                                    dim3(kThreads), params, smem, stream, kPair ? 2 : 1));
