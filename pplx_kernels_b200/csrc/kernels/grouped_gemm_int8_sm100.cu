@@ -105,9 +105,14 @@ __device__ __forceinline__ float scaled(uint32_t sum, float sx, float sw) {
   return static_cast<float>(static_cast<int32_t>(sum)) * sx * sw;
 }
 
-// silu(gate) * up; the quotient by the hardware's reciprocal (2 steps of fp32 off).
+// silu(gate) * up by t = exp(-|gate|), which is at most 1: gate / (1 + t), and gate * t / (1 + t) for
+// negative gates.  The reciprocal is the hardware's (one step of fp32 off); its argument lies in (1, 2], so
+// no gate leaves its range (1 + exp(-gate) would, for gates below -87.33).
 __device__ __forceinline__ float swiglu(float gate, float up) {
-  return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+  const float t = __expf(-fabsf(gate));
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + t));
+  return (gate < 0.0f ? gate * t : gate) * inv * up;
 }
 
 __device__ __forceinline__ uint32_t pack(float a, float b, bool fp16) {
