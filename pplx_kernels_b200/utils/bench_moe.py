@@ -119,6 +119,18 @@ def verify_layer(layer, fp8: bool, x: torch.Tensor, idx: torch.Tensor, w: torch.
     return "fused and composed against the PyTorch reference over all experts, and against each other"
 
 
+def _figures(times: dict, tokens: int, floors: dict, floor: float) -> dict:
+    """What is reported of the forms that ran, from their times in us."""
+    fused = {"fused_frac_of_roofline": floor / times["fused"]} if "fused" in times else {}
+    return {
+        **{f"{name}_us_p50": t for name, t in times.items()},
+        **{f"{name}_tokens_per_s": tokens / (t * 1e-6) for name, t in times.items()},
+        "floors_us": floors,
+        **fused,
+        "best_frac_of_roofline": floor / min(times.values()),
+    }
+
+
 def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: int,
             dev: torch.device, zipf: float = 0.0, graph: bool = False,
             flush: torch.Tensor | None = None, fp8: bool = False, replays: int = 1,
@@ -179,7 +191,6 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
         res[name] = float(t.median())
     layer.check_status()
     layer.destroy()
-    res.setdefault("fused", res["composed"])  # (a layer with one form)
 
     peaks = _peaks()
     # Per GPU: rows = tokens * top-k (uniform routing, weak scaling)
@@ -201,7 +212,6 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
     }
     floor = max(floors["compute_us"], floors["weights_hbm_us"],
                 floors["nvlink_dispatch_us"] + floors["nvlink_combine_us"])
-    best = min(res["fused"], res["composed"])
     return {
         "model": cfg.name,
         "dtype": ("fp8 block-scaled, power-of-two scales applied by the tensor cores"
@@ -210,12 +220,7 @@ def measure(model: str, tokens: int, iters: int, warmup: int, rank: int, world: 
         "n_gpus": world,
         "tokens_per_gpu": m, "graph": graph, "replays_per_sample": replays if graph else 1,
         "zipf": zipf, "output_checked": checked,
-        "composed_us_p50": res["composed"], "fused_us_p50": res["fused"],
-        "fused_tokens_per_s": world * m / (res["fused"] * 1e-6),
-        "composed_tokens_per_s": world * m / (res["composed"] * 1e-6),
-        "floors_us": floors,
-        "fused_frac_of_roofline": floor / res["fused"],
-        "best_frac_of_roofline": floor / best,
+        **_figures(res, world * m, floors, floor),
     }
 
 
