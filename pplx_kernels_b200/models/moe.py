@@ -350,7 +350,11 @@ class MoELayerInt8:
         grouped_gemm_int8(self.expert_x[:n], self.expert_scale[:n], self.w13_q, self.w13_s,
                           rows.counts, rows.offsets, swiglu=True, out=self.h[:n],
                           status=self.gemm_status, expected_rows=expect)
-        quantize_rows_int8(self.h[:n], out=self.h_q[:n], out_scale=self.h_scale[:n])
+        if bound_m is None:
+            quantize_rows_int8(self.h[:n], out=self.h_q[:n], out_scale=self.h_scale[:n])
+        else:  # (rows behind the last expert's hold what an earlier call left)
+            quantize_rows_int8(self.h[:n].unsqueeze(0), rows.offsets[-1:],
+                               out=self.h_q[:n].unsqueeze(0), out_scale=self.h_scale[:n].unsqueeze(0))
         grouped_gemm_int8(self.h_q[:n], self.h_scale[:n], self.w2_q, self.w2_s, rows.counts,
                           rows.offsets, out=self.expert_y[:n], status=self.gemm_status,
                           expected_rows=expect)
