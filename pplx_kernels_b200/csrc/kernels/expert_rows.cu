@@ -757,6 +757,13 @@ void with_type(FloatType type, int bytes, Fn&& fn) {
 // us, and the next kernel finds them in L2.)
 bool stream_past_l2(int64_t bytes) { return bytes > (int64_t{126} << 20); }
 
+// Rows that a call writes (or reads) at most: of a table with a capacity only those that entries of the
+// routing have, unless the others are cleared.  (1024 tokens of 7168 bf16, top-6, to 64 x 512 rows, 470 MB
+// of which 88 are written, and back: 32.2 us past L2, 29.4 through it; in 8 bits 12.0, 11.5.)
+int64_t touched_rows(const ExpertRowsView& r, bool zero_rest) {
+  return zero_rest ? r.num_rows : std::min(r.num_rows, static_cast<int64_t>(r.num_tokens) * r.topk);
+}
+
 int size_of(FloatType t) { return t == FloatType::kFloat ? 4 : 2; }
 
 }  // namespace
@@ -787,7 +794,7 @@ void launch_sort_by_expert(const SortByExpertCall& c, cudaStream_t stream) {
 
 void launch_permute_tokens(const PermuteCall& call, cudaStream_t stream) {
   PermuteCall c = call;
-  c.streaming = stream_past_l2((c.rows.num_tokens + c.rows.num_rows) * c.row_bytes);
+  c.streaming = stream_past_l2((c.rows.num_tokens + touched_rows(c.rows, c.zero_rest)) * c.row_bytes);
   const int64_t items = c.rows.num_tokens + (c.zero_rest ? c.rows.num_rows : 0);
   if (items == 0 || c.row_bytes == 0) return;
   const int vec = alignment(16, {address(c.x), address(c.out), static_cast<uint64_t>(c.row_bytes),
@@ -805,8 +812,8 @@ void launch_permute_tokens(const PermuteCall& call, cudaStream_t stream) {
 
 void launch_unpermute_tokens(const UnpermuteCall& call, cudaStream_t stream) {
   UnpermuteCall c = call;
-  c.streaming = stream_past_l2((c.rows.num_tokens * static_cast<int64_t>(c.rows.topk + 1)) * c.hidden *
-                               size_of(c.type));
+  c.streaming =
+      stream_past_l2((c.rows.num_tokens + touched_rows(c.rows, false)) * c.hidden * size_of(c.type));
   if (c.rows.num_tokens == 0 || c.hidden == 0) return;
   const uint64_t size = size_of(c.type);
   const int vec = alignment(16, {address(c.y), address(c.out), c.hidden * size, c.out_stride * size});
@@ -854,9 +861,13 @@ void launch_quantize_rows(const QuantizeRowsCall& call, cudaStream_t stream) {
   QuantizeRowsCall c = call;
   ExpertRowsView r{};
   if (c.rows != nullptr) r = *c.rows;
-  c.streaming = stream_past_l2(c.rows != nullptr
-                                   ? (r.num_rows + r.num_tokens * static_cast<int64_t>(size_of(c.type))) * c.hidden
-                                   : c.num_rows * (1 + size_of(c.type)) * c.hidden);
+  // (Only the device knows how many counted rows there are.  32 x 1024 rows of 2048, us past L2 and not, all
+  // live 30.9, 31.8, quantised twice and read back 105.5, 103.3; 32 live each 7.8, 7.8.)
+  if (c.rows != nullptr)
+    c.streaming = stream_past_l2(
+        (touched_rows(r, c.zero_rest) + r.num_tokens * static_cast<int64_t>(size_of(c.type))) * c.hidden);
+  else
+    c.streaming = c.counts == nullptr && stream_past_l2(c.num_rows * (1 + size_of(c.type)) * c.hidden);
   const int64_t items = (c.rows != nullptr ? r.num_tokens : c.num_rows) +
                         (c.zero_rest ? r.num_rows : 0);
   if (items == 0) return;
