@@ -49,17 +49,30 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                : "memory");
 }
 
+// kTensorMemory: for arrivals by mbar_arrive_on_leader_relaxed, see there.
+template <bool kTensorMemory = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t done;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred P;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P;\n\t"
-      "}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+  if constexpr (kTensorMemory)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
   return done != 0;
 }
 
@@ -75,9 +88,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // working warps of the CTA need.  How long a sleep in vain lasts is up to the hardware (0.07 to
 // 0.7 ms were measured), so the limit is read off the clock, after such a sleep.  (Modulo 2^32 ns,
 // with an odd end so that 0 can say that there is none yet: a wide clock cost registers.)
+template <bool kTensorMemory = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
                                            volatile uint32_t* abort_flag, uint32_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_try_wait<kTensorMemory>(bar, parity)) return true;
   constexpr uint32_t kSleepNs = 1000000;
   uint32_t end = 0;
 #pragma unroll 1
@@ -92,7 +106,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
         : "=r"(done)
         : "r"(smem_u32(bar)), "r"(parity), "r"(kSleepNs)
         : "memory");
-    if (done != 0u) return true;
+    // (The sleep only watches the phase; what orders the arrivals behind it is the same look as above.)
+    if (done != 0u && (!kTensorMemory || mbar_try_wait<kTensorMemory>(bar, parity))) return true;
     if (*abort_flag != 0u) return false;
     uint32_t now;
     asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
@@ -187,8 +202,14 @@ __device__ __forceinline__ void mbar_arrive_on_leader(uint64_t* bar) {
                : "memory");
 }
 
-// The same for a thread that has nothing to publish but that its tensor-memory loads are over
-// (tcgen05.wait::ld): a release would also wait for its stores to global memory, about 1400 cycles.
+// The same for a warp that hands back tensor memory it has read, and nothing else.  Its loads are over when
+// tcgen05.wait::ld returns; tcgen05.fence::before_thread_sync orders them before the arrival, and
+// tcgen05.fence::after_thread_sync the next MMAs behind the wait that sees it.  This is the pattern that the PTX
+// ISA manual gives for tcgen05 instructions of different threads (tcgen05 memory consistency model,
+// canonical synchronization patterns): the two fences around an mbarrier arrival and wait that are
+// themselves .relaxed.cluster.  No ordinary memory is passed on this way.  A release at cluster scope would
+// also wait for the warp's stores to global memory, about 1400 cycles: 128 experts of 768 x 2048 (down), 256
+// rows each 63.4 -> 72.4 us, 8 of 256 x 14336, 1024 rows 97 -> 113 us.
 __device__ __forceinline__ void mbar_arrive_on_leader_relaxed(uint64_t* bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                    smem_u32(bar) & kPeerBitMask)

@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc1 = tc::make_instr_desc_i8(kBlockM * kCtas, n1);
         const uint32_t slot0 = slot, lap0 = lap;
         next_slot();
-        ok = tc::mbar_wait(&ctl->tmem_empty[slot0], lap0 ^ 1u, abort_flag, kWaitLimitNs);
+        ok = tc::mbar_wait<kPair>(&ctl->tmem_empty[slot0], lap0 ^ 1u, abort_flag, kWaitLimitNs);
         if (!ok) break;
         tc::tc_fence_after_sync();
         // One half's MMAs of a K block.
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t stage1 = stage, phase1 = phase;
         bool free1 = false;
         for (int kb0 = 0, kb1 = 0; kb1 < num_kb;) {
-          if (!free1 && tc::mbar_try_wait(&ctl->tmem_empty[slot1], lap1 ^ 1u)) {
+          if (!free1 && tc::mbar_try_wait<kPair>(&ctl->tmem_empty[slot1], lap1 ^ 1u)) {
             free1 = true;
             tc::tc_fence_after_sync();
           }
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             next_stage(stage, phase);
             if (++kb0 == num_kb) commit(&ctl->tmem_full[slot0]);
           } else {
-            ok = tc::mbar_wait(&ctl->tmem_empty[slot1], lap1 ^ 1u, abort_flag, kWaitLimitNs);
+            ok = tc::mbar_wait<kPair>(&ctl->tmem_empty[slot1], lap1 ^ 1u, abort_flag, kWaitLimitNs);
             if (!ok) break;
           }
         }
