@@ -15,18 +15,19 @@
 // to 512, of which each CTA loads half (wide tiles as two halves that share the weights).  No TMA
 // multicast is involved.
 //
-// What bounds it, at 6.5 TB/s of HBM and 3.36 POPS (twice the bf16 rate): the weights' bytes up to
-// some 128 rows per expert (32 experts of 2048 x 7168, up projection, 64 rows each: 145 us, floor 147
-// with the rows), L2 around 256 rows (175 us, floor 158), the tensor cores and the power limit above
-// (1024 rows: 600 us = 3.2 POPS; 8 experts of 4096 x 14336, down, 1024 rows: 296 us).  An epilogue that
-// divided by the IEEE quotient and met two barriers per 16 tokens bound the tiles with short K: 128
-// experts of 768 x 2048, up, 256 rows 191 us, now 91; down 77 -> 65.
+// What bounds it (cards differ by their power limit, 5 to 10 % from 256 rows per expert on): the weights'
+// bytes up to some 128 rows per expert (32 experts of 2048 x 7168, up projection, 64 rows each: 142 to 150 us, 6.4
+// to 6.8 TB/s with the rows); L2 around 256 rows (255 rows: 185 us alone, 158 by the bytes, 142 by the
+// operations at twice the bf16 rate, 3.36 POPS); the tensor cores and the power limit above (1024 rows: 600
+// to 700 us, 2.8 to 3.2 POPS; 8 experts of 4096 x 14336, down, 1024 rows: 295 to 350 us).  An epilogue that divided by the IEEE quotient and
+// met two barriers per 16 tokens bound the tiles with short K: 128 experts of 768 x 2048, up, 256 rows 191
+// us, now 93; down 77 -> 62.
 //
 // Roles (persistent over tiles): warp 0 TMA producer, warp 1 MMA issuer (leader CTA only), warp 2
 // tensor-memory allocation, warps 4-11 epilogue.  Two accumulators of 256 columns let the epilogue
-// of a tile run under the MMAs of the next; for wider tiles see below.  Every mbarrier wait is bounded: when one runs out the CTA raises a
-// shared abort flag, all roles leave their loops, in-flight TMA loads are drained, tensor memory is
-// freed and the kernel returns with *status = 1.
+// of a tile run under the MMAs of the next; for wider tiles see below.  Every mbarrier wait is bounded:
+// when one runs out the CTA raises a shared abort flag, all roles leave their loops, in-flight TMA loads
+// are drained, tensor memory is freed and the kernel returns with *status = 1.
 #include <algorithm>
 
 #include <cuda.h>

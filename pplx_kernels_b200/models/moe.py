@@ -276,6 +276,9 @@ class MoELayerInt8:
     are quantised, dispatched as 8-bit payload with one scale each, and combined like those of the
     other layers.  The intermediate is rounded to bf16 by the up projection before it is quantised:
     its row's largest value is known only when the whole row is.
+
+    Calls share the layer's buffers: forward passes, replays of captured ones too, run one after the
+    other (on one stream, or ordered by events).  Nothing is recorded for a backward pass.
     """
 
     def __init__(self, cfg: MoEModelConfig, max_num_tokens: int, rank: int = 0,
