@@ -442,29 +442,42 @@ void check_no_tangent(const at::Tensor& t, const char* op, const char* name) {
               " carries a tangent; forward-mode derivatives are not implemented");
 }
 
-// What operators without a gradient of their own do in place of recording one.  A tensor that is written
-// counts as changed, so that a backward pass that saved it notices; one that a gradient is recorded for
-// is refused, as by torch's own `out=`.
+// fn(tensor, argument) for the tensors on the stack that `schema` describes.
+template <typename F>
+void for_tensors(const c10::FunctionSchema& schema, const torch::jit::Stack& stack, F&& fn) {
+  const size_t n = schema.arguments().size(), first = stack.size() - n;
+  for (size_t i = 0; i < n; ++i)
+    if (stack[first + i].isTensor() && stack[first + i].toTensor().defined())
+      fn(stack[first + i].toTensor(), schema.arguments()[i]);
+}
+
+bool is_written(const c10::Argument& argument) {
+  return argument.alias_info() != nullptr && argument.alias_info()->isWrite();
+}
+
+// What operators without a gradient of their own do in place of recording one.  A written tensor that a
+// gradient is recorded for is refused, as by torch's own `out=`.
 void not_differentiable(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
                         torch::jit::Stack* stack) {
-  const c10::FunctionSchema& schema = op.schema();
-  const char* name = schema.name().c_str() + schema.name().rfind(':') + 1;
-  c10::SmallVector<at::Tensor, 4> written;
-  const size_t n = schema.arguments().size(), first = stack->size() - n;
-  for (size_t i = 0; i < n; ++i) {
-    const c10::IValue& v = (*stack)[first + i];
-    if (!v.isTensor() || !v.toTensor().defined()) continue;
-    const at::Tensor& t = v.toTensor();
-    const c10::Argument& argument = schema.arguments()[i];
+  const char* name = op.schema().name().c_str() + op.schema().name().rfind(':') + 1;
+  for_tensors(op.schema(), *stack, [&](const at::Tensor& t, const c10::Argument& argument) {
     check_no_tangent(t, name, argument.name().c_str());
-    if (argument.alias_info() == nullptr || !argument.alias_info()->isWrite()) continue;
-    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, ": ", argument.name(),
+    TORCH_CHECK(!(is_written(argument) && t.requires_grad() && at::GradMode::is_enabled()), name, ": ",
+                argument.name(),
                 " is written and requires a gradient, which is not recorded; use torch.no_grad() or detach()");
-    written.push_back(t);
-  }
+  });
   op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
-  for (const at::Tensor& t : written)
-    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
+// Written tensors count as changed, so that a backward pass that saved them notices (in inference mode as
+// well, where only tensors made there have no version).
+void count_changes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  c10::SmallVector<at::Tensor, 4> written;
+  for_tensors(op.schema(), *stack, [&](const at::Tensor& t, const c10::Argument& argument) {
+    if (is_written(argument) && !t.is_inference()) written.push_back(t);
+  });
+  op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
+  for (const at::Tensor& t : written) torch::autograd::impl::bump_version(t);
 }
 
 at::Tensor permute_tokens_autograd(const at::Tensor& x, const at::Tensor& counts,
@@ -700,6 +713,10 @@ void register_expert_ops(torch::Library& m) {
                          "quantize_rows_int8_out", "grouped_gemm_int8"})
     m.impl(op, c10::DispatchKey::Autograd,
            torch::CppFunction::makeFromBoxedFunction<&not_differentiable>());
+  for (const char* op : {"permute_tokens_out", "permute_tokens_int8_out", "unpermute_tokens_out",
+                         "unpermute_tokens_backward", "quantize_rows_int8_out", "grouped_gemm_int8"})
+    m.impl(op, c10::DispatchKey::ADInplaceOrView,
+           torch::CppFunction::makeFromBoxedFunction<&count_changes>());
 }
 
 }  // namespace pplx

@@ -182,3 +182,12 @@ def test_scales_of_a_product_that_require_a_gradient_are_refused():
             product(*scales)
         with torch.no_grad():
             assert product(*scales).shape == (E, 4, 16)
+
+
+@pytest.mark.parametrize("name", WRITING)
+def test_written_tensors_count_as_changed_in_inference_mode(name):
+    written = {"copy": [0], "sum": [0], "product": [3, 4]}.get(name, [1, 2])
+    o = buffers()
+    with torch.inference_mode():
+        WRITING[name](o)
+    assert [t._version for t in o] == [int(i in written) for i in range(5)]
